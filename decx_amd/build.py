@@ -26,7 +26,8 @@ HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibilit
              # feature and says "ignoring feature" once per module: harmless, and dropped from the output below.
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
              "-Wno-unused-command-line-argument"]
-HIP_SOURCES = ["gemm_f32.hip", "gemm_f32_dma.hip", "gemm_f16.hip", "gemm_f16_dma.hip", "gemm_f64.hip", "gemm_complex.hip", "gemv.hip", "conv_direct.hip", "capi.hip"]
+HIP_SOURCES = ["gemm_f32.hip", "gemm_f32_dma.hip", "gemm_f16.hip", "gemm_f16_dma.hip", "gemm_f64.hip", "gemm_complex.hip", "gemv.hip", "conv_direct.hip",
+               "gemm_q4.hip", "q4_pack.hip", "rmsnorm.hip", "capi.hip"]
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wextra",
               "-I" + os.path.join(ROOT, "include")]
 

@@ -3,6 +3,7 @@
 #include "../../include/decx_hip.h"
 #include "../../include/decx_hip_profiling.h"
 #include "gemm_common.hpp"
+#include "gemm_q4.hpp"
 #include "split_k_exchange.hpp"
 #include "split_counter_ring.hpp"
 
@@ -1197,6 +1198,157 @@ int decx_hip_conv2d_f32_depth(const float* image, const float* kmat, float* dst,
     g.conv_image_bytes = ((uint64_t)(out_h - 1) * stride_y + k_h) * img_wpitch * img_dpitch * 4u;
     if (conv2d_direct_pays(g.N, g.K, img_dpitch, depth)) return launch_conv2d_direct_f32(g, img_dpitch, depth, as_stream(stream));
     return launch_conv2d_f32_dma(choose_tile(false, g.M, g.N, true), g, as_stream(stream));
+}
+
+// ---- weights in 4 bits, and the norm in front of them
+
+static bool q4_shape_ok(uint32_t N, uint32_t K, uint32_t group)
+{
+    if (group != 32 && group != 64 && group != 128) return false;
+    const uint64_t tiles = (uint64_t)(N / kQ4TileRows + (N % kQ4TileRows != 0)) * (K / kQ4TileCols + (K % kQ4TileCols != 0));
+    return K <= 0xffffff00u && N <= 0xffffff00u && tiles <= 0x7fffffffu;     // (offsets past the last column, and a grid of tiles)
+}
+static inline bool aligned_to(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+// codes are read 16 bytes at a time, the scales and zero points of a tile's row together
+static bool q4_parts_ok(const void* codes, const void* scales, const void* zeros, uint32_t group)
+{
+    const uintptr_t per_tile = kQ4TileCols / group;
+    return codes && scales && aligned16(codes) && aligned_to(scales, 2 * per_tile) && (!zeros || aligned_to(zeros, per_tile));
+}
+
+size_t decx_hip_q4_codes_bytes(uint32_t N, uint32_t K)
+{
+    return (size_t)(N / kQ4TileRows + (N % kQ4TileRows != 0)) * (K / kQ4TileCols + (K % kQ4TileCols != 0)) * kQ4TileBytes;
+}
+
+size_t decx_hip_q4_scales_count(uint32_t N, uint32_t K, uint32_t group)
+{
+    if (group != 32 && group != 64 && group != 128) return 0;
+    return decx_hip_q4_codes_bytes(N, K) / kQ4TileBytes * kQ4TileRows * (kQ4TileCols / group);
+}
+
+static int run_q4_quantize(bool f16, const void* W, void* codes, uint16_t* scales, uint8_t* zeros, uint32_t N, uint32_t K, uint32_t ldw,
+                           uint32_t group, void* stream)
+{
+    const bool empty = N == 0 || K == 0;
+    if (!q4_shape_ok(N, K, group) ||
+        (!empty && (!W || ldw < K || !aligned_to(W, f16 ? 2 : 4) || !q4_parts_ok(codes, scales, zeros, group))))
+        return DECX_HIP_E_INVALID_ARG;
+    if (!g_dev.ready) return DECX_HIP_E_NOT_INIT;
+    if (empty) return DECX_HIP_OK;
+    return launch_q4_quantize(f16, W, N, K, ldw, group, codes, scales, zeros, as_stream(stream));
+}
+
+int decx_hip_q4_quantize_f32(const float* W, void* codes, uint16_t* scales, uint8_t* zeros, uint32_t N, uint32_t K, uint32_t ldw,
+                             uint32_t group, void* stream)
+{
+    return run_q4_quantize(false, W, codes, scales, zeros, N, K, ldw, group, stream);
+}
+int decx_hip_q4_quantize_f16(const uint16_t* W, void* codes, uint16_t* scales, uint8_t* zeros, uint32_t N, uint32_t K, uint32_t ldw,
+                             uint32_t group, void* stream)
+{
+    return run_q4_quantize(true, W, codes, scales, zeros, N, K, ldw, group, stream);
+}
+
+static int run_q4_dequantize(bool f16, const void* codes, const uint16_t* scales, const uint8_t* zeros, void* W, uint32_t N, uint32_t K,
+                             uint32_t ldw, uint32_t group, void* stream)
+{
+    const bool empty = N == 0 || K == 0;
+    if (!q4_shape_ok(N, K, group) ||
+        (!empty && (!W || ldw < K || !aligned_to(W, f16 ? 2 : 4) || !q4_parts_ok(codes, scales, zeros, group))))
+        return DECX_HIP_E_INVALID_ARG;
+    if (!g_dev.ready) return DECX_HIP_E_NOT_INIT;
+    if (empty) return DECX_HIP_OK;
+    return launch_q4_dequantize(f16, codes, scales, zeros, W, N, K, ldw, group, as_stream(stream));
+}
+
+int decx_hip_q4_dequantize_f32(const void* codes, const uint16_t* scales, const uint8_t* zeros, float* W, uint32_t N, uint32_t K,
+                               uint32_t ldw, uint32_t group, void* stream)
+{
+    return run_q4_dequantize(false, codes, scales, zeros, W, N, K, ldw, group, stream);
+}
+int decx_hip_q4_dequantize_f16(const void* codes, const uint16_t* scales, const uint8_t* zeros, uint16_t* W, uint32_t N, uint32_t K,
+                               uint32_t ldw, uint32_t group, void* stream)
+{
+    return run_q4_dequantize(true, codes, scales, zeros, W, N, K, ldw, group, stream);
+}
+
+static int run_gemm_q4(bool i8, const void* X, const float* x_scales, const void* codes, const uint16_t* scales, const uint8_t* zeros,
+                       const void* C, void* Y, uint32_t M, uint32_t N, uint32_t K, uint32_t group, uint32_t ldx, uint32_t ldc, uint32_t ldy,
+                       float alpha, float beta, int y_is_f32, void* workspace, size_t workspace_bytes, void* stream)
+{
+    (void)workspace; (void)workspace_bytes;
+    const bool empty = M == 0 || N == 0;
+    const uintptr_t y_bytes = y_is_f32 ? 4 : 2;
+    if (!q4_shape_ok(N, K, group)) return DECX_HIP_E_INVALID_ARG;
+    if (empty) return g_dev.ready ? DECX_HIP_OK : DECX_HIP_E_NOT_INIT;
+    if (!Y || ldy < N || !aligned_to(Y, y_bytes) || (C && ((ldc != 0 && ldc < N) || !aligned_to(C, y_bytes))) || M > 0xffffff00u)
+        return DECX_HIP_E_INVALID_ARG;
+    if (K > 0 && (!X || ldx < K || (!i8 && !aligned_to(X, 2)) || !q4_parts_ok(codes, scales, zeros, group))) return DECX_HIP_E_INVALID_ARG;
+    if (i8 && (!x_scales || !aligned_to(x_scales, 4))) return DECX_HIP_E_INVALID_ARG;
+    if (!g_dev.ready) return DECX_HIP_E_NOT_INIT;
+    GemmQ4Args g;
+    std::memset(&g, 0, sizeof g);
+    g.X = X; g.x_scales = x_scales;
+    g.codes = (const unsigned char*)codes; g.scales = (const _Float16*)scales; g.zeros = zeros;
+    g.C = C; g.Y = Y;
+    g.M = M; g.N = N; g.K = K;
+    g.ldx = ldx; g.ldc = ldc; g.ldy = ldy;
+    g.alpha = alpha; g.beta = beta;
+    g.y_f32 = y_is_f32 ? 1 : 0;
+    g.k_tiles = (K + kQ4TileCols - 1) / kQ4TileCols;
+    g.n_tiles = (N + kQ4TileRows - 1) / kQ4TileRows;
+    return launch_gemm_q4(i8, group, g, as_stream(stream));
+}
+
+int decx_hip_gemm_q4_f16(const uint16_t* X, const void* codes, const uint16_t* scales, const uint8_t* zeros, const void* C, void* Y,
+                         uint32_t M, uint32_t N, uint32_t K, uint32_t group, uint32_t ldx, uint32_t ldc, uint32_t ldy, float alpha, float beta,
+                         int y_is_f32, void* workspace, size_t workspace_bytes, void* stream)
+{
+    return run_gemm_q4(false, X, nullptr, codes, scales, zeros, C, Y, M, N, K, group, ldx, ldc, ldy, alpha, beta, y_is_f32, workspace,
+                       workspace_bytes, stream);
+}
+int decx_hip_gemm_q4_i8(const int8_t* X, const float* x_scales, const void* codes, const uint16_t* scales, const uint8_t* zeros, const void* C,
+                        void* Y, uint32_t M, uint32_t N, uint32_t K, uint32_t group, uint32_t ldx, uint32_t ldc, uint32_t ldy, float alpha,
+                        float beta, int y_is_f32, void* workspace, size_t workspace_bytes, void* stream)
+{
+    return run_gemm_q4(true, X, x_scales, codes, scales, zeros, C, Y, M, N, K, group, ldx, ldc, ldy, alpha, beta, y_is_f32, workspace,
+                       workspace_bytes, stream);
+}
+
+size_t decx_hip_gemm_q4_workspace(int x_is_i8, uint32_t M, uint32_t N, uint32_t K, uint32_t group)
+{
+    (void)x_is_i8; (void)M; (void)N; (void)K; (void)group;
+    return 0;
+}
+
+static int run_rmsnorm(bool f16, const void* x, const void* residual, const void* weight, void* sum, void* y, float* y_scales, uint32_t rows,
+                       uint32_t cols, uint32_t ldx, uint32_t ldr, uint32_t lds, uint32_t ldy, float eps, void* stream)
+{
+    const uintptr_t e = f16 ? 2 : 4;
+    if (rows == 0) return g_dev.ready ? DECX_HIP_OK : DECX_HIP_E_NOT_INIT;
+    if (!x || !weight || !y || cols == 0 || cols > 0xffff0000u || rows > 0x7fffffffu || ldx < cols || (residual && ldr < cols) ||
+        (sum && lds < cols) || ldy < cols || !(eps >= 0.f) || !aligned_to(x, e) || !aligned_to(residual, e) || !aligned_to(weight, e) ||
+        !aligned_to(sum, e) || (!y_scales && !aligned_to(y, e)) || !aligned_to(y_scales, 4))
+        return DECX_HIP_E_INVALID_ARG;
+    if (!g_dev.ready) return DECX_HIP_E_NOT_INIT;
+    RmsNormArgs g;
+    std::memset(&g, 0, sizeof g);
+    g.x = x; g.residual = residual; g.weight = weight; g.sum = sum; g.y = y; g.y_scales = y_scales;
+    g.rows = rows; g.cols = cols; g.ldx = ldx; g.ldr = ldr; g.lds = lds; g.ldy = ldy;
+    g.eps = eps;
+    return launch_rmsnorm(f16, g, as_stream(stream));
+}
+
+int decx_hip_rmsnorm_f16(const uint16_t* x, const uint16_t* residual, const uint16_t* weight, uint16_t* sum, void* y, float* y_scales,
+                         uint32_t rows, uint32_t cols, uint32_t ldx, uint32_t ldr, uint32_t lds, uint32_t ldy, float eps, void* stream)
+{
+    return run_rmsnorm(true, x, residual, weight, sum, y, y_scales, rows, cols, ldx, ldr, lds, ldy, eps, stream);
+}
+int decx_hip_rmsnorm_f32(const float* x, const float* residual, const float* weight, float* sum, void* y, float* y_scales, uint32_t rows,
+                         uint32_t cols, uint32_t ldx, uint32_t ldr, uint32_t lds, uint32_t ldy, float eps, void* stream)
+{
+    return run_rmsnorm(false, x, residual, weight, sum, y, y_scales, rows, cols, ldx, ldr, lds, ldy, eps, stream);
 }
 
 int decx_hip_gemm_plan(int elem_bytes, uint32_t M, uint32_t N, uint32_t K, int aligned, decx_hip_plan* out)

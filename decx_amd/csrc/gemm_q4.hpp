@@ -1,0 +1,50 @@
+// Shared declarations of the 4-bit layer: products with weights held in 4 bits, the step that makes such weights, and
+// the root-mean-square norm in front of them.
+#pragma once
+#include "gemm_common.hpp"
+
+namespace decx_hip {
+
+// Where a 4-bit matrix of N rows x K columns keeps its parts.  Tiles of 16 rows x 128 columns, 1024 bytes each,
+// [row tile][column tile]: one 16-byte piece per lane of a wavefront in the order the matrix instruction wants its
+// operand, so that a wavefront's load of a tile is 1 KB in a row and no code changes lanes on its way.  Lane 16 kg + r
+// holds row r; word j of its piece the columns 32 j + 8 kg + 0..7, in nibbles 0, 4, 1, 5, 2, 6, 3, 7: masking the word
+// with 0x000f000f (0x00f000f0, ...) then gives two adjacent columns in two halves.  Scales and zero points lie
+// [row tile][column tile][row][group of the tile].
+constexpr uint32_t kQ4TileRows = 16, kQ4TileCols = 128, kQ4TileBytes = 1024;
+
+struct GemmQ4Args {
+    const void* X;               // fp16 or int8, M x K
+    const float* x_scales;       // int8: a factor per row of X
+    const unsigned char* codes;
+    const _Float16* scales;
+    const unsigned char* zeros;  // or null: 8 everywhere
+    const void* C;               // of Y's type, or null; ldc = 0: one row for all
+    void* Y;                     // fp16, or fp32 with y_f32
+    uint32_t M, N, K;
+    uint32_t ldx, ldc, ldy;
+    float alpha, beta;
+    uint32_t y_f32;
+    uint32_t k_tiles, n_tiles;   // tiles along K and N
+};
+
+int launch_gemm_q4(bool i8, uint32_t group, const GemmQ4Args& args, hipStream_t stream);
+
+int launch_q4_quantize(bool f16, const void* W, uint32_t N, uint32_t K, uint32_t ldw, uint32_t group, void* codes, void* scales,
+                       void* zeros, hipStream_t stream);
+int launch_q4_dequantize(bool f16, const void* codes, const void* scales, const void* zeros, void* W, uint32_t N, uint32_t K,
+                         uint32_t ldw, uint32_t group, hipStream_t stream);
+
+struct RmsNormArgs {
+    const void* x;
+    const void* residual;        // or null
+    const void* weight;
+    void* sum;                   // x + residual, or null
+    void* y;                     // rows' type, or int8 with y_scales
+    float* y_scales;
+    uint32_t rows, cols, ldx, ldr, lds, ldy;
+    float eps;
+};
+int launch_rmsnorm(bool f16, const RmsNormArgs& args, hipStream_t stream);
+
+}  // namespace decx_hip

@@ -70,6 +70,17 @@ SYMBOLS = {
     "decx_hip_conv2d_pack_kernels_f32": (_int, [_vp, _vp] + [_u32] * 5 + [ctypes.c_uint64] + [_u32] * 3 + [_vp]),
     "decx_hip_conv2d_f32": (_int, [_vp] * 3 + [_u32] * 12 + [_vp]),
     "decx_hip_conv2d_f32_depth": (_int, [_vp] * 3 + [_u32] * 13 + [_vp]),
+    "decx_hip_q4_codes_bytes": (_sz, [_u32] * 2),
+    "decx_hip_q4_scales_count": (_sz, [_u32] * 3),
+    "decx_hip_q4_quantize_f32": (_int, [_vp] * 4 + [_u32] * 4 + [_vp]),
+    "decx_hip_q4_quantize_f16": (_int, [_vp] * 4 + [_u32] * 4 + [_vp]),
+    "decx_hip_q4_dequantize_f32": (_int, [_vp] * 4 + [_u32] * 4 + [_vp]),
+    "decx_hip_q4_dequantize_f16": (_int, [_vp] * 4 + [_u32] * 4 + [_vp]),
+    "decx_hip_gemm_q4_workspace": (_sz, [_int] + [_u32] * 4),
+    "decx_hip_gemm_q4_f16": (_int, [_vp] * 6 + [_u32] * 7 + [_f, _f, _int, _vp, _sz, _vp]),
+    "decx_hip_gemm_q4_i8": (_int, [_vp] * 7 + [_u32] * 7 + [_f, _f, _int, _vp, _sz, _vp]),
+    "decx_hip_rmsnorm_f16": (_int, [_vp] * 6 + [_u32] * 6 + [_f, _vp]),
+    "decx_hip_rmsnorm_f32": (_int, [_vp] * 6 + [_u32] * 6 + [_f, _vp]),
     "decx_hip_gemm_f64": (_int, [_vp] * 4 + [_u32] * 7 + [ctypes.c_double, ctypes.c_double, _vp]),
     "decx_hip_gemm_f64_tile": (_int, [_vp] * 4 + [_u32] * 7 + [ctypes.c_double, ctypes.c_double, _vp, _int, _int]),
     "decx_hip_gemm_complex_workspace": (ctypes.c_size_t, [_int, _u32, _u32]),
@@ -274,6 +285,68 @@ def gevm(x, B, y, c=None, alpha=1.0, beta=1.0, stream=None, workspace=None):
         fn = L.decx_hip_gevm_f32 if workspace is None else L.decx_hip_gevm_f32_ws
         rc = fn(xp, B.ptr, cp, yp, K, N, B.pitch, incx, incc, incy, alpha, beta, *ws, stream)
     check(rc, "gevm")
+
+
+class Q4Matrix:
+    """A matrix of rows x cols (N x K) held in 4 bits on the device: codes, scales and, with zeros=True, zero points in the
+    layout of include/decx_hip.h.  Made from a DeviceMatrix by quantize_q4."""
+
+    def __init__(self, rows, cols, group=128, zeros=False):
+        L = lib()
+        self.rows, self.cols, self.group = rows, cols, group
+        count = L.decx_hip_q4_scales_count(rows, cols, group)
+        self.codes = DeviceMatrix(1, max(L.decx_hip_q4_codes_bytes(rows, cols), 16), np.uint8)
+        self.scales = DeviceMatrix(1, max(count, 1), np.float16)
+        self.zeros = DeviceMatrix(1, max(count, 1), np.uint8) if zeros else None
+
+    def parts(self):
+        return self.codes.ptr, self.scales.ptr, self.zeros.ptr if self.zeros is not None else None
+
+
+def quantize_q4(W, Q, stream=None):
+    """Fills the Q4Matrix Q from the DeviceMatrix W (fp32 or fp16) of its size."""
+    assert (W.rows, W.cols) == (Q.rows, Q.cols) and W.dtype in (np.float32, np.float16)
+    fn = lib().decx_hip_q4_quantize_f16 if W.dtype == np.float16 else lib().decx_hip_q4_quantize_f32
+    check(fn(W.ptr, *Q.parts(), Q.rows, Q.cols, W.pitch, Q.group, stream), "quantize_q4")
+
+
+def dequantize_q4(Q, W, stream=None):
+    """The values that Q stands for, into the DeviceMatrix W (fp32 or fp16) of its size."""
+    assert (W.rows, W.cols) == (Q.rows, Q.cols) and W.dtype in (np.float32, np.float16)
+    fn = lib().decx_hip_q4_dequantize_f16 if W.dtype == np.float16 else lib().decx_hip_q4_dequantize_f32
+    check(fn(*Q.parts(), W.ptr, Q.rows, Q.cols, W.pitch, Q.group, stream), "dequantize_q4")
+
+
+def gemm_q4(X, Q, Y, C=None, alpha=1.0, beta=1.0, x_scales=None, workspace=None, stream=None):
+    """Y = X . Q^T or fma(C, beta, alpha * X . Q^T) on DeviceMatrix operands; X fp16, or int8 with x_scales (M fp32 values);
+    C of one row is added to every row of Y when Y has more."""
+    M, N, K = X.rows, Q.rows, Q.cols
+    assert X.cols == K and (Y.rows, Y.cols) == (M, N) and Y.dtype in (np.float16, np.float32)
+    if C is not None:
+        assert C.dtype == Y.dtype and C.cols == N and C.rows in (1, M)
+    ldc = 0 if C is None or (C.rows == 1 and M > 1) else C.pitch
+    ws = (None, 0) if workspace is None else (workspace.ptr, workspace.rows * workspace.pitch * workspace.dtype.itemsize)
+    rest = (*Q.parts(), C.ptr if C is not None else None, Y.ptr, M, N, K, Q.group, X.pitch, ldc, Y.pitch, alpha, beta,
+            1 if Y.dtype == np.float32 else 0, *ws, stream)
+    if X.dtype == np.int8:
+        assert x_scales is not None and x_scales.dtype == np.float32 and x_scales.rows * x_scales.cols == M
+        rc = lib().decx_hip_gemm_q4_i8(X.ptr, x_scales.ptr, *rest)
+    else:
+        assert X.dtype == np.float16 and x_scales is None
+        rc = lib().decx_hip_gemm_q4_f16(X.ptr, *rest)
+    check(rc, "gemm_q4")
+
+
+def rmsnorm(x, weight, y, residual=None, sum_out=None, y_scales=None, eps=1e-5, stream=None):
+    """y = h * weight / sqrt(mean(h^2) + eps) row by row, h = x + residual (kept in sum_out); y int8 with y_scales, or of x's type."""
+    assert x.dtype in (np.float16, np.float32) and weight.dtype == x.dtype and weight.cols == x.cols
+    assert y.dtype == (np.int8 if y_scales is not None else x.dtype)
+    for o in (y, residual, sum_out):
+        assert o is None or (o.rows, o.cols) == (x.rows, x.cols)
+    fn = lib().decx_hip_rmsnorm_f16 if x.dtype == np.float16 else lib().decx_hip_rmsnorm_f32
+    p = lambda m: (m.ptr, m.pitch) if m is not None else (None, 0)                          # noqa: E731
+    check(fn(x.ptr, p(residual)[0], weight.ptr, p(sum_out)[0], y.ptr, p(y_scales)[0], x.rows, x.cols, x.pitch, p(residual)[1], p(sum_out)[1],
+             y.pitch, eps, stream), "rmsnorm")
 
 
 def _align(v, a):

@@ -296,6 +296,79 @@ DECX_HIP_API int decx_hip_conv2d_f32_depth(const float* image, const float* kmat
                                            uint32_t stride_x, uint32_t stride_y,
                                            uint32_t kmat_pitch, uint32_t dst_dpitch, uint32_t dst_wpitch, void* stream);
 
+/* ---- weights in 4 bits, and the norm in front of them ---------------------------------------
+ * The reference has no counterpart: these serve a trained linear layer beside the products above.
+ *
+ * A 4-bit matrix W (N x K) in groups of `group` = 32, 64 or 128 columns stands for
+ *
+ *   W(n, k) = (code(n, k) - zero(n, k / group)) * scale(n, k / group)        code, zero in 0..15
+ *
+ * and consists of three device arrays, all in tiles of 16 rows x 128 columns, [row tile][column tile] (the last ones
+ * padded; what the padding of codes holds is never used):
+ *   codes   decx_hip_q4_codes_bytes(N, K) bytes, 16-byte aligned, 1024 a tile.  In a tile the 32-bit word
+ *           [kg 0..3][row 0..15][j 0..3] holds columns 32 j + 8 kg + 0..7, in its nibbles 0, 4, 1, 5, 2, 6, 3, 7
+ *           (nibble 0: the lowest four bits): the order in which the matrix instruction takes them;
+ *   scales  decx_hip_q4_scales_count(N, K, group) fp16 values, [row 0..15][group of the tile] in a tile; aligned to the
+ *           scales of one row of a tile (256 / group bytes);
+ *   zeros   as many bytes in the same order, aligned to 128 / group, or NULL: 8 everywhere. */
+DECX_HIP_API size_t decx_hip_q4_codes_bytes(uint32_t N, uint32_t K);
+DECX_HIP_API size_t decx_hip_q4_scales_count(uint32_t N, uint32_t K, uint32_t group);   /* 0 for any other group */
+
+/* Makes a 4-bit matrix of W (N x K, row pitch ldw).  Per group, over its columns that exist:
+ *   zeros == NULL:  scale = max|w| / 7,  code = clamp(rint(w / scale), -8, 7) + 8
+ *   otherwise:      lo = min(0, min w), hi = max(0, max w), scale = (hi - lo) / 15, zero = clamp(rint(-lo / scale), 0, 15),
+ *                   code = clamp(rint(w / scale) + zero, 0, 15)
+ * with the scale computed in fp32, at most 65504, and rounded to fp16, the rounded one being divided by; halves round to
+ * even and no quotient's rounding decides a code.  A group whose scale rounds to zero holds code = zero = 8; one that
+ * holds a NaN or an infinity gets scale NaN. */
+DECX_HIP_API int decx_hip_q4_quantize_f32(const float* W, void* codes, uint16_t* scales, uint8_t* zeros, uint32_t N, uint32_t K,
+                                          uint32_t ldw, uint32_t group, void* stream);
+DECX_HIP_API int decx_hip_q4_quantize_f16(const uint16_t* W, void* codes, uint16_t* scales, uint8_t* zeros, uint32_t N, uint32_t K,
+                                          uint32_t ldw, uint32_t group, void* stream);
+/* The values a 4-bit matrix stands for (exact in fp32; rounded once to fp16). */
+DECX_HIP_API int decx_hip_q4_dequantize_f32(const void* codes, const uint16_t* scales, const uint8_t* zeros, float* W, uint32_t N,
+                                            uint32_t K, uint32_t ldw, uint32_t group, void* stream);
+DECX_HIP_API int decx_hip_q4_dequantize_f16(const void* codes, const uint16_t* scales, const uint8_t* zeros, uint16_t* W, uint32_t N,
+                                            uint32_t K, uint32_t ldw, uint32_t group, void* stream);
+
+/* Y (M x N) = X (M x K) . W^T                       when C == NULL
+ * Y         = fma(C, beta, alpha * (X . W^T))       otherwise
+ * for a 4-bit W.  M = 1 is the matrix x vector product of a single token, bound by reading the codes; M of thousands runs
+ * at the rate of the matrix cores.  X is fp16, or int8 where row m stands for X(m, :) * x_scales[m] (what
+ * decx_hip_rmsnorm_* writes).  C and Y are fp16, or both fp32 when y_is_f32 != 0; ldc = 0 adds the one row C to every row
+ * of Y (a bias); C may be Y.  Products are of X with the whole number code - zero, summed over a group in fp32 (int8: in
+ * int32, exactly) before the scale meets them; sums are fp32, Y is rounded once.  Bases and pitches of X, C and Y need
+ * only be whole elements.  workspace: device memory that lets ranges of K be multiplied by workgroups of their own
+ * where the output alone would leave CUs idle; NULL or too small is never an error, the sums then run in one piece.
+ * decx_hip_gemm_q4_workspace says how many bytes are of use (0: none).  It must be 16-byte aligned and is free again when
+ * the call's work on `stream` is done; calls that may overlap -- other streams, graphs replayed side by side -- each need
+ * their own.  Results do not depend on timing, but may differ in rounding with and without it. */
+DECX_HIP_API size_t decx_hip_gemm_q4_workspace(int x_is_i8, uint32_t M, uint32_t N, uint32_t K, uint32_t group);
+DECX_HIP_API int decx_hip_gemm_q4_f16(const uint16_t* X, const void* codes, const uint16_t* scales, const uint8_t* zeros,
+                                      const void* C, void* Y, uint32_t M, uint32_t N, uint32_t K, uint32_t group,
+                                      uint32_t ldx, uint32_t ldc, uint32_t ldy, float alpha, float beta, int y_is_f32,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+DECX_HIP_API int decx_hip_gemm_q4_i8(const int8_t* X, const float* x_scales, const void* codes, const uint16_t* scales,
+                                     const uint8_t* zeros, const void* C, void* Y, uint32_t M, uint32_t N, uint32_t K,
+                                     uint32_t group, uint32_t ldx, uint32_t ldc, uint32_t ldy, float alpha, float beta, int y_is_f32,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Root-mean-square norm of `rows` rows of `cols` elements:
+ *   h = x + residual (residual == NULL: x), rounded to the rows' type and written to `sum` unless that is NULL
+ *   y = h * weight / sqrt(mean(h^2) + eps)
+ * y_scales == NULL: y in the rows' type.  Otherwise y holds int8 codes and y_scales one factor per row:
+ *   top = max |h * weight|,  code = rint(127 * h * weight / top),  y_scales = top / (127 sqrt(mean(h^2) + eps)) -- the rows
+ * decx_hip_gemm_q4_i8 takes.  A row of zeros has scale 0; one that meets a NaN or an infinity has codes 0 and scale NaN.
+ * sum may be x or residual, and y (in the rows' type) any of the three, at the same pitch; other overlaps are not allowed.
+ * Pitches in elements (of y: in elements of its own type), at least cols; any alignment of whole elements.  Sums of squares
+ * are kept in fp32 (fp32 rows: 64 bits).  cols = 0 and a negative eps are refused. */
+DECX_HIP_API int decx_hip_rmsnorm_f16(const uint16_t* x, const uint16_t* residual, const uint16_t* weight, uint16_t* sum,
+                                      void* y, float* y_scales, uint32_t rows, uint32_t cols, uint32_t ldx, uint32_t ldr,
+                                      uint32_t lds, uint32_t ldy, float eps, void* stream);
+DECX_HIP_API int decx_hip_rmsnorm_f32(const float* x, const float* residual, const float* weight, float* sum,
+                                      void* y, float* y_scales, uint32_t rows, uint32_t cols, uint32_t ldx, uint32_t ldr,
+                                      uint32_t lds, uint32_t ldy, float eps, void* stream);
+
 /* Same as decx_hip_gemm_f32 / _f16 with the planner's choice overridden (`tile` = one of
  * DECX_HIP_TILE_*; AUTO = planner) and, with force_edge != 0, the predicated kernel
  * variant forced even for shapes that are tile multiples.  For tests and tuning. */
