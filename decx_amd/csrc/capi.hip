@@ -1277,7 +1277,7 @@ static int run_gemm_q4(bool i8, const void* X, const float* x_scales, const void
                        const void* C, void* Y, uint32_t M, uint32_t N, uint32_t K, uint32_t group, uint32_t ldx, uint32_t ldc, uint32_t ldy,
                        float alpha, float beta, int y_is_f32, void* workspace, size_t workspace_bytes, void* stream)
 {
-    (void)workspace; (void)workspace_bytes;
+    (void)workspace_bytes;
     const bool empty = M == 0 || N == 0;
     const uintptr_t y_bytes = y_is_f32 ? 4 : 2;
     if (!q4_shape_ok(N, K, group)) return DECX_HIP_E_INVALID_ARG;
@@ -1296,8 +1296,10 @@ static int run_gemm_q4(bool i8, const void* X, const float* x_scales, const void
     g.ldx = ldx; g.ldc = ldc; g.ldy = ldy;
     g.alpha = alpha; g.beta = beta;
     g.y_f32 = y_is_f32 ? 1 : 0;
+    g.workspace = workspace;
     g.k_tiles = (K + kQ4TileCols - 1) / kQ4TileCols;
     g.n_tiles = (N + kQ4TileRows - 1) / kQ4TileRows;
+    g.quads_ok = (ldy % 4 == 0 && aligned_to(Y, 4 * y_bytes) && (!C || (ldc % 4 == 0 && aligned_to(C, 4 * y_bytes)))) ? 1 : 0;
     return launch_gemm_q4(i8, group, g, as_stream(stream));
 }
 

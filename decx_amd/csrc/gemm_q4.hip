@@ -7,6 +7,10 @@
 // multiplied by its scale, in fp32: no product of code and scale is ever rounded to 16 bits.
 #include "gemm_q4.hpp"
 #include "split_k_exchange.hpp"
+#ifdef Q4_EXPERIMENT
+#include <cstdlib>
+#include <cstdio>
+#endif
 
 namespace decx_hip {
 
@@ -20,51 +24,77 @@ typedef uintx2 uintx2_u __attribute__((aligned(1)));
 __device__ __forceinline__ halfx2 as_half2(uint32_t w) { return __builtin_bit_cast(halfx2, w); }
 
 // Eight codes of a word less the zero point, as fp16.  A code in the low bits of 0x6400 reads 1024 + code, in bits 4..7
-// 1024 + 16 code; both steps back are exact in fp16.
-struct ZeroF16 { halfx2 low, high; };                     // -(1024 + zero), -(64 + zero), twice each
-__device__ __forceinline__ ZeroF16 zero_f16(uint32_t z)
-{
-    const _Float16 low = (_Float16)(float)-(int)(1024 + z), high = (_Float16)(float)-(int)(64 + z);
-    return {halfx2{low, low}, halfx2{high, high}};
-}
-__device__ __forceinline__ halfx8 widen_f16(uint32_t w, const ZeroF16& z)
-{
-    const halfx2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
-    const uint32_t v = w >> 8;
-    const halfx2 a = as_half2((w & 0x000f000fu) | 0x64006400u) + z.low;
-    const halfx2 b = __builtin_elementwise_fma(as_half2((w & 0x00f000f0u) | 0x64006400u), sixteenth, z.high);
-    const halfx2 c = as_half2((v & 0x000f000fu) | 0x64006400u) + z.low;
-    const halfx2 d = __builtin_elementwise_fma(as_half2((v & 0x00f000f0u) | 0x64006400u), sixteenth, z.high);
-    return halfx8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-// The same as int8, columns in the order 0, 4, 1, 5 | 2, 6, 3, 7.  zero: the zero point in every byte.
-__device__ __forceinline__ uintx2 widen_i8(uint32_t w, uint32_t zero)
-{
-    const uint32_t low = ((w & 0x0f0f0f0fu) | 0x80808080u) - zero, high = (((w >> 4) & 0x0f0f0f0fu) | 0x80808080u) - zero;
-    return uintx2{low ^ 0x80808080u, high ^ 0x80808080u};
-}
+// 1024 + 16 code; the steps back are exact in fp16, and so are their constants: -(1024 + zero) is 0xe400 + zero,
+// -(64 + zero) 0xd400 + 16 zero.  (The masks are kept in registers: from there mask and exponent are one instruction.)
+struct WidenF16 {
+    uint32_t first, second, exponent;
+    __device__ __forceinline__ WidenF16() : first(0x000f000fu), second(0x00f000f0u), exponent(0x64006400u)
+    {
+        asm("" : "+s"(first), "+s"(second), "+v"(exponent));
+    }
+    struct Zero { halfx2 low, high; };
+    static __device__ __forceinline__ Zero zero(uint32_t z) { return {as_half2(z * 0x00010001u + 0xe400e400u), as_half2(z * 0x00100010u + 0xd400d400u)}; }
+    __device__ __forceinline__ halfx8 operator()(uint32_t w, const Zero& z) const
+    {
+        const halfx2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
+        const uint32_t v = w >> 8;
+        const halfx2 a = as_half2((w & first) | exponent) + z.low;
+        const halfx2 b = __builtin_elementwise_fma(as_half2((w & second) | exponent), sixteenth, z.high);
+        const halfx2 c = as_half2((v & first) | exponent) + z.low;
+        const halfx2 d = __builtin_elementwise_fma(as_half2((v & second) | exponent), sixteenth, z.high);
+        return halfx8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    }
+};
+// The same as int8, columns in the order 0, 4, 1, 5 | 2, 6, 3, 7.  With zero points (in every byte of `zero`): code - zero.
+// Without: 16 (code - 8), the code in the upper half of its byte (FACTOR, taken back with the scale).
+template <bool ZEROS> struct WidenI8 {
+    uint32_t mask, sign;
+    __device__ __forceinline__ WidenI8() : mask(ZEROS ? 0x0f0f0f0fu : 0xf0f0f0f0u), sign(ZEROS ? 0x80808080u : 0x88888888u)
+    {
+        asm("" : "+s"(mask), "+v"(sign));
+    }
+    __device__ __forceinline__ uintx2 operator()(uint32_t w, uint32_t zero) const
+    {
+        if constexpr (ZEROS) {
+            const uint32_t low = ((w & mask) | sign) - zero, high = (((w >> 4) & mask) | sign) - zero;
+            return uintx2{low ^ sign, high ^ sign};
+        } else {
+            const uint32_t v = w ^ sign;
+            return uintx2{(v << 4) & mask, v & mask};
+        }
+    }
+};
+template <bool I8, bool ZEROS> struct Factor { static constexpr float value = I8 && !ZEROS ? 0.0625f : 1.f; };
 // Eight int8 of X in that order.
 __device__ __forceinline__ uintx2 order_i8(uintx2 x)
 {
     return uintx2{__builtin_amdgcn_perm(x[1], x[0], 0x05010400u), __builtin_amdgcn_perm(x[1], x[0], 0x07030602u)};
 }
 
-// Columns k..k+7 of a row of X, zero from K on.
-__device__ __forceinline__ halfx8 load_x8(const _Float16* row, uint32_t k, uint32_t K)
+// 16 bytes of a row from column k on, zero from column K on (for the last column tile; K >= 1): the 16 bytes that end at K,
+// shifted down, so that one load does and nothing behind the row is read.
+template <typename T> __device__ __forceinline__ uintx4 load_end(const T* row, uint32_t k, uint32_t K)
 {
-    if (k + 8 <= K) return *(const halfx8_u*)(row + k);
-    halfx8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) if (k + e < K) v[e] = row[k + e];
-    return v;
-}
-__device__ __forceinline__ uintx2 load_x8(const signed char* row, uint32_t k, uint32_t K)
-{
-    if (k + 8 <= K) return *(const uintx2_u*)(row + k);
-    uintx2 v = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) if (k + e < K) v[e / 4] |= (uint32_t)(unsigned char)row[k + e] << (8 * (e % 4));
-    return v;
+    constexpr uint32_t E = 16 / sizeof(T);
+    uint64_t low = 0, high = 0;
+    if (k < K && K >= E) {
+        const uint32_t first = k + E <= K ? k : K - E, shift = (k - first) * 8 * sizeof(T);
+        uintx4 v;
+        __builtin_memcpy(&v, row + first, 16);
+        low = (uint64_t)v[1] << 32 | v[0];
+        high = (uint64_t)v[3] << 32 | v[2];
+        if (shift >= 64) { low = high >> (shift - 64); high = 0; }
+        else { low = low >> shift | high << 1 << (63 - shift); high >>= shift; }
+    } else if (k < K) {
+#pragma unroll 1
+        for (uint32_t e = 0; k + e < K; ++e) {             // (rows shorter than that)
+            typename std::conditional<sizeof(T) == 1, uint8_t, uint16_t>::type bits;
+            __builtin_memcpy(&bits, row + k + e, sizeof(T));
+            const uint32_t at = e * 8 * sizeof(T);
+            if (at < 64) low |= (uint64_t)bits << at; else high |= (uint64_t)bits << (at - 64);
+        }
+    }
+    return uintx4{(uint32_t)low, (uint32_t)(low >> 32), (uint32_t)high, (uint32_t)(high >> 32)};
 }
 
 template <int GPB> struct Scales { typedef _Float16 type __attribute__((ext_vector_type(GPB))); };
@@ -86,99 +116,226 @@ __device__ __forceinline__ void store_y(const GemmQ4Args& g, uint32_t m, uint32_
     else ((_Float16*)g.Y)[at] = (_Float16)v;
 }
 
+// Four adjacent outputs of a row, the first of them inside.
+__device__ __forceinline__ void store_y4(const GemmQ4Args& g, uint32_t m, uint32_t n, floatx4 v)
+{
+    if (n + 4 > g.N || !g.quads_ok) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (n + e < g.N) store_y(g, m, n + e, v[e]);
+        return;
+    }
+    if (g.x_scales) {
+        const float s = g.x_scales[m];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] *= s;
+    }
+    if (g.C) {
+        const size_t at = (size_t)m * g.ldc + n;
+        floatx4 c;
+        if (g.y_f32) {
+            c = *(const floatx4*)((const float*)g.C + at);
+        } else {
+            const halfx4 h = *(const halfx4*)((const _Float16*)g.C + at);
+            c = floatx4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(c[e], g.beta, g.alpha * v[e]);
+    }
+    const size_t at = (size_t)m * g.ldy + n;
+    if (g.y_f32) *(floatx4*)((float*)g.Y + at) = v;
+    else *(halfx4*)((_Float16*)g.Y + at) = halfx4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+}
+
 }  // namespace
 
+// X in LDS: rows of one column tile of W, 128 columns.  fp16: 256 bytes, 16-byte chunk c (columns 8 c ..) of row r in slot
+// c ^ (r % 16).  int8: 128 bytes, chunk 4 s + kg holding the two pieces of 8 columns from 64 s + 8 kg and from 64 s + 32 + 8 kg,
+// each in the codes' order, in slot chunk ^ (r / 2 % 8).  So a lane's operand of a matrix instruction is one 16-byte read, and
+// the 16 rows that a quarter of a wavefront reads together cover all banks.
+template <bool I8> struct XRows {
+    static constexpr int BYTES = I8 ? 128 : 256, CHUNKS = BYTES / 16;
+    // where the 16 bytes `at` (of CHUNKS, in the order of memory) of a row go
+    static __device__ __forceinline__ uint32_t place(int row, int at)
+    {
+        if constexpr (I8) {
+            // their two pieces of 8 columns belong to block j = at / 2 of 32 columns and to kg = at % 2 * 2 + (0, 1); s = j / 2, half j % 2
+            const int chunk = at / 4 * 4 + at % 2 * 2;
+            return row * BYTES + ((chunk ^ ((row >> 1) & 7)) * 16) + (at / 2 % 2) * 8;
+        } else {
+            return row * BYTES + ((at ^ (row & 15)) * 16);
+        }
+    }
+    static __device__ __forceinline__ void put(unsigned char* lds, uint32_t place, const uintx4& v)
+    {
+        if constexpr (I8) {
+            // (the second piece's chunk is the next one: the first is even, so its slot differs in the lowest bit)
+            *(uintx2*)(lds + place) = order_i8(uintx2{v[0], v[1]});
+            *(uintx2*)(lds + (place ^ 16)) = order_i8(uintx2{v[2], v[3]});
+        } else {
+            *(uintx4*)(lds + place) = v;
+        }
+    }
+    // chunk: 4 j + kg (fp16, step j of 32 columns), 4 s + kg (int8, step s of 64); row16: the row in its tile of 16
+    static __device__ __forceinline__ uint32_t slot(int chunk, int row16) { return (chunk ^ (I8 ? (row16 >> 1) & 7 : row16)) * 16; }
+};
+
+// ---- few rows --------------------------------------------------------------------------------------------------------
+//
 // A workgroup owns T row tiles of W (16 T columns of Y) and 16 TM rows of X; its wavefronts deal the column tiles of W among
-// themselves and their sums meet in LDS, in wavefront order.  GPB: groups per column tile (128 / group).
-template <bool I8, int GPB, int TM, int T, int WAVES>
+// themselves and their sums meet in LDS, in wavefront order.  The codes go straight into the registers the matrix instruction
+// reads, 1 KB of a tile a load, one step ahead of the products.  X comes out of the L2, where every wavefront reads other
+// columns of it.  Read in the instruction's order, 16 rows of 64 bytes a load, it would keep the L1 busy with lines; so a
+// wavefront loads whole rows (4 of 256 bytes at a time) and turns them around in LDS of its own, which nobody waits for.
+template <bool I8, int GPB, bool ZEROS, int TM, int T, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64)
+__attribute__((amdgpu_waves_per_eu(TM == 1 ? 4 : 2)))
 gemm_q4_rows_kernel(const GemmQ4Args g)
 {
     typedef typename std::conditional<I8, signed char, _Float16>::type X_t;
-    __shared__ float red[WAVES][T * TM][4][64];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l16 = lane & 15, kg = lane >> 4;
+    typedef typename std::conditional<I8, intx4, floatx4>::type P_t;
+    typedef typename Scales<GPB>::type S_t;
+    typedef XRows<I8> R;
+    constexpr int TURN_BYTES = 16 * TM * R::BYTES, CH = TURN_BYTES / 1024, ROWS_AT_ONCE = 64 / R::CHUNKS;
+    constexpr int RED_BYTES = WAVES * T * TM * 1024;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[WAVES * TURN_BYTES > RED_BYTES ? WAVES * TURN_BYTES : RED_BYTES];
+    float (*const red)[T * TM][4][64] = (float (*)[T * TM][4][64])lds;
+    const int t = threadIdx.x, lane = t & 63, l16 = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const uint32_t tile0 = blockIdx.x * T, m0 = blockIdx.y * (16 * TM);
 
-    const X_t* row[TM];
-    bool has[TM];
+    unsigned char* const turn = lds + wave * TURN_BYTES;
+    const int turn_row = lane / R::CHUNKS, turn_at = lane % R::CHUNKS;
+    const unsigned char* const turn_src = (const unsigned char*)g.X + (size_t)(m0 + turn_row < g.M ? m0 + turn_row : 0) * g.ldx * sizeof(X_t);
+    const size_t turn_step = (size_t)ROWS_AT_ONCE * g.ldx * sizeof(X_t);
+    uintx4 turning[CH];
+    const auto fetch_rows = [&](uint32_t kt) {
+        if ((kt + 1) * kQ4TileCols <= g.K) {               // (the columns of a part of a tile are fetched as they are turned)
+            const unsigned char* const src = turn_src + ((size_t)kt * kQ4TileCols * sizeof(X_t) + turn_at * 16);
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const uint32_t m = m0 + 16 * i + l16;
-        has[i] = m < g.M;
-        row[i] = (const X_t*)g.X + (size_t)(has[i] ? m : 0) * g.ldx;
-    }
+            for (int c = 0; c < CH; ++c)
+                if (m0 + turn_row + c * ROWS_AT_ONCE < g.M)    // (rows behind the last one: whatever LDS holds, they are not stored)
+                    __builtin_memcpy(&turning[c], src + c * turn_step, 16);
+        }
+    };
+    const auto turn_rows = [&](uint32_t kt) {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if ((kt + 1) * kQ4TileCols <= g.K) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) R::put(turn, R::place(turn_row + c * ROWS_AT_ONCE, turn_at), turning[c]);
+        } else {
+#pragma unroll 1
+            for (int c = 0; c < CH; ++c)
+                if (m0 + turn_row + c * ROWS_AT_ONCE < g.M)
+                    R::put(turn, R::place(turn_row + c * ROWS_AT_ONCE, turn_at),
+                           load_end((const X_t*)(turn_src + c * turn_step), kt * kQ4TileCols + turn_at * (16 / sizeof(X_t)), g.K));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+
+    size_t tile_at[T];
+#pragma unroll
+    for (int c = 0; c < T; ++c) tile_at[c] = (size_t)(tile0 + c < g.n_tiles ? tile0 + c : g.n_tiles - 1) * g.k_tiles;
+
+    struct Codes { uintx4 w[T]; S_t s[T]; uint32_t z[T]; };
+    const auto fetch_codes = [&](Codes& f, uint32_t kt) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < T; ++c) {
+            const size_t tile = tile_at[c] + kt;
+            f.w[c] = *(const uintx4*)(g.codes + tile * kQ4TileBytes + lane * 16);
+            f.s[c] = *(const S_t*)(g.scales + (tile * 16 + l16) * GPB);
+            f.z[c] = 0x08080808u;
+            if constexpr (ZEROS) f.z[c] = *(const typename Zeros<GPB>::type*)(g.zeros + (tile * 16 + l16) * GPB);
+        }
+    };
+    const WidenF16 widen_f16;
+    const WidenI8<ZEROS> widen_i8;
     floatx4 acc[T][TM];
 #pragma unroll
     for (int c = 0; c < T; ++c)
 #pragma unroll
         for (int i = 0; i < TM; ++i) acc[c][i] = floatx4{0, 0, 0, 0};
+    const auto multiply = [&](const Codes& f, uint32_t kt) __attribute__((always_inline)) {
+        constexpr int STEPS = 4 / GPB;                     // words of a group
+        static_for<0, GPB>([&](auto qc) {
+            constexpr int q = decltype(qc)::value;
+            P_t part[T][TM], none = {0, 0, 0, 0};
+            asm volatile("" : "+v"(none));                 // (one quad of zeros, not one for every product)
+            float s[T];
+            WidenF16::Zero zf[T];
+            uint32_t zi[T];
+#pragma unroll
+            for (int c = 0; c < T; ++c) {
+                if constexpr (GPB == 1) s[c] = (float)f.s[c]; else s[c] = (float)f.s[c][q];
+                s[c] *= Factor<I8, ZEROS>::value;
+                if (kt * kQ4TileCols + q * (kQ4TileCols / GPB) >= g.K) s[c] = 0.f;       // a group beyond the last column
+                const uint32_t z = (f.z[c] >> (8 * q)) & 0xffu;
+                zf[c] = WidenF16::zero(z);
+                zi[c] = z * 0x01010101u;
+            }
+            // words taken together: two of an int8 group (64 columns), one otherwise
+            constexpr int BY = I8 && STEPS > 1 ? 2 : 1;
+            static_for<0, STEPS / BY>([&](auto jc) {
+                constexpr int j = q * STEPS + decltype(jc)::value * BY;
+                uintx4 x[TM];
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+                    x[i] = *(const uintx4*)(turn + (16 * i + l16) * R::BYTES + R::slot((I8 ? j / 2 : j) * 4 + kg, l16));
+                    if constexpr (I8 && BY == 1 && j % 2) { x[i][0] = x[i][2]; x[i][1] = x[i][3]; }
+                }
+#pragma unroll
+                for (int c = 0; c < T; ++c) {
+                    if constexpr (!I8) {
+                        const halfx8 wf = widen_f16(f.w[c][j], zf[c]);
+#pragma unroll
+                        for (int i = 0; i < TM; ++i)
+                            part[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, x[i]), wf, decltype(jc)::value == 0 ? none : part[c][i], 0, 0, 0);
+                    } else if constexpr (BY == 1) {
+                        const uintx2 wi = widen_i8(f.w[c][j], zi[c]);
+#pragma unroll
+                        for (int i = 0; i < TM; ++i)
+                            part[c][i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, uintx2{x[i][0], x[i][1]}), __builtin_bit_cast(long, wi), none, 0, 0, 0);
+                    } else {
+                        const uintx2 w0 = widen_i8(f.w[c][j], zi[c]), w1 = widen_i8(f.w[c][j + 1], zi[c]);
+                        const intx4 b = {(int)w0[0], (int)w0[1], (int)w1[0], (int)w1[1]};
+#pragma unroll
+                        for (int i = 0; i < TM; ++i)
+                            part[c][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(intx4, x[i]), b, decltype(jc)::value == 0 ? none : part[c][i], 0, 0, 0);
+                    }
+                }
+            });
+#pragma unroll
+            for (int c = 0; c < T; ++c)
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[c][i][e] = __builtin_fmaf((float)part[c][i][e], s[c], acc[c][i][e]);
+                    asm volatile("" : "+v"(acc[c][i]));    // (here and now: put off to where acc is next needed, the parts would live until then)
+                }
+        });
+    };
 
-    for (uint32_t kt = wave; kt < g.k_tiles; kt += WAVES) {
-        const uint32_t k0 = kt * kQ4TileCols + 8 * kg;
-        halfx8 xf[TM][4];
-        uintx2 xi[TM][4];
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (I8) {
-                    xi[i][j] = uintx2{0, 0};
-                    if (has[i]) xi[i][j] = order_i8(load_x8(row[i], k0 + 32 * j, g.K));
-                } else {
-                    xf[i][j] = halfx8{0, 0, 0, 0, 0, 0, 0, 0};
-                    if (has[i]) xf[i][j] = load_x8(row[i], k0 + 32 * j, g.K);
-                }
-            }
-#pragma unroll
-        for (int c = 0; c < T; ++c) {
-            const uint32_t nt = tile0 + c < g.n_tiles ? tile0 + c : g.n_tiles - 1;
-            const size_t tile = (size_t)nt * g.k_tiles + kt;
-            const uintx4 w = *(const uintx4*)(g.codes + tile * kQ4TileBytes + lane * 16);
-            const size_t at = (tile * 16 + l16) * GPB;
-            const typename Scales<GPB>::type sv = *(const typename Scales<GPB>::type*)(g.scales + at);
-            uint32_t zv = 0x08080808u;
-            if (g.zeros) zv = *(const typename Zeros<GPB>::type*)(g.zeros + at);
-#pragma unroll
-            for (int q = 0; q < GPB; ++q) {
-                constexpr int STEPS = 4 / GPB;             // words of a group
-                float s;
-                if constexpr (GPB == 1) s = (float)sv; else s = (float)sv[q];
-                if (kt * kQ4TileCols + q * (kQ4TileCols / GPB) >= g.K) s = 0.f;       // a group beyond the last column
-                const uint32_t z = (zv >> (8 * q)) & 0xffu;
-                if constexpr (I8) {
-                    const uint32_t zz = z * 0x01010101u;
-#pragma unroll
-                    for (int i = 0; i < TM; ++i) {
-                        intx4 part = {0, 0, 0, 0};
-                        if constexpr (STEPS == 1) {
-                            part = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, xi[i][q]), __builtin_bit_cast(long, widen_i8(w[q], zz)), part, 0, 0, 0);
-                        } else {
-#pragma unroll
-                            for (int j = q * STEPS; j < (q + 1) * STEPS; j += 2) {
-                                const uintx2 w0 = widen_i8(w[j], zz), w1 = widen_i8(w[j + 1], zz);
-                                const intx4 a = {(int)xi[i][j][0], (int)xi[i][j][1], (int)xi[i][j + 1][0], (int)xi[i][j + 1][1]};
-                                const intx4 b = {(int)w0[0], (int)w0[1], (int)w1[0], (int)w1[1]};
-                                part = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, part, 0, 0, 0);
-                            }
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[c][i][e] = __builtin_fmaf((float)part[e], s, acc[c][i][e]);
-                    }
-                } else {
-                    const ZeroF16 zz = zero_f16(z);
-#pragma unroll
-                    for (int i = 0; i < TM; ++i) {
-                        floatx4 part = {0, 0, 0, 0};
-#pragma unroll
-                        for (int j = q * STEPS; j < (q + 1) * STEPS; ++j)
-                            part = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[i][j], widen_f16(w[j], zz), part, 0, 0, 0);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[c][i][e] = __builtin_fmaf(part[e], s, acc[c][i][e]);
-                    }
-                }
-            }
+    // codes for two steps, taking turns
+    Codes a, b;
+    uint32_t kt = wave;
+    const auto step = [&](const Codes& now, Codes& next) __attribute__((always_inline)) {
+        turn_rows(kt);
+        if (kt + WAVES < g.k_tiles) {
+            fetch_codes(next, kt + WAVES);
+            fetch_rows(kt + WAVES);
         }
+        multiply(now, kt);
+        kt += WAVES;
+        return kt < g.k_tiles;
+    };
+    if (kt < g.k_tiles) {
+        fetch_codes(a, kt);
+        fetch_rows(kt);
+        while (step(a, b) && step(b, a)) {}
     }
+    __syncthreads();
     // lane (kg, l16) holds rows 4 kg .. 4 kg + 3 of X and row l16 of W of every 16 x 16 piece
 #pragma unroll
     for (int c = 0; c < T; ++c)
@@ -198,26 +355,305 @@ gemm_q4_rows_kernel(const GemmQ4Args g)
     }
 }
 
+// ---- many rows -------------------------------------------------------------------------------------------------------
+//
+// A workgroup owns BM = 16 TM WM rows of X and BN = 16 TN WN columns of Y; a wavefront (wm, wn) of it 16 TM x 16 TN.  X goes
+// through LDS, one column tile of W (128 of K) per stage, two stages; its global loads travel through registers, so that they
+// may be unaligned and int8 can be put into the order of the codes on the way.  The codes need no LDS: a wavefront loads the
+// pieces of its TN row tiles straight into the registers the matrix instruction reads them from, one stage ahead, and
+// widens them there, once for all its TM tiles of X.
+template <bool I8, int GPB, bool ZEROS, int TM, int TN, int WM, int WN>
+__global__ void __launch_bounds__(WM * WN * 64)
+__attribute__((amdgpu_waves_per_eu(TM * TN >= 32 ? 1 : 2)))
+gemm_q4_tiles_kernel(const GemmQ4Args g)
+{
+    constexpr int NT = WM * WN * 64, BM = 16 * TM * WM, BN = 16 * TN * WN;
+    typedef XRows<I8> R;
+    typedef typename std::conditional<I8, signed char, _Float16>::type X_t;
+    constexpr int ROW = R::BYTES, CPR = R::CHUNKS, STAGE = BM * ROW, CH = STAGE / 16 / NT;
+    constexpr int STEPS = 4 / GPB, GROUP = 128 / GPB;
+    constexpr int EPI = WM * WN * 16 * 16 * TN * 4;
+    static_assert(CH >= 1 && CH * NT * 16 == STAGE, "whole chunks per thread");
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * STAGE > EPI ? 2 * STAGE : EPI];
+    typedef typename Scales<GPB>::type S_t;
+
+    const int t = threadIdx.x, lane = t & 63, l16 = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wm = wave / WN, wn = wave % WN;
+    uint32_t tile_m, tile_n, z;
+    {
+        // every XCD a contiguous range of tiles, walked in groups of 4 tile rows (gemm_common.hpp, block_to_tile)
+        const uint32_t tiles = g.tiles_m * g.tiles_n;
+        z = blockIdx.x / tiles;
+        GemmArgs map;
+        map.tiles_m = g.tiles_m; map.tiles_n = g.tiles_n; map.group_m = 0;
+        block_to_tile(map, blockIdx.x % tiles, tiles, 0, tile_m, tile_n);
+    }
+    const uint32_t m0 = tile_m * BM, n0 = tile_n * BN;
+    const uint32_t kt0 = z * g.split_tiles, kt1 = kt0 + g.split_tiles < g.k_tiles ? kt0 + g.split_tiles : g.k_tiles;
+
+    // ---- X: chunk c of this thread is the 16 bytes `at` of row `row`
+    const unsigned char* src[CH];
+    uint32_t dst[CH];
+    const int at = t % CPR;                                // (NT is a multiple of the chunks of a row)
+    static_assert(NT % CPR == 0, "");
+    const auto row_of = [&](int c) {
+        const uint32_t m = m0 + t / CPR + c * (NT / CPR);
+        return (const unsigned char*)g.X + (size_t)(m < g.M ? m : g.M - 1) * g.ldx * (I8 ? 1 : 2);       // rows behind the last one: never stored
+    };
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        src[c] = row_of(c) + at * 16;
+        dst[c] = R::place(t / CPR + c * (NT / CPR), at);
+    }
+    uintx4 staged[CH];
+    const auto fetch_x = [&](uint32_t kt) {
+        if ((kt + 1) * 128 <= g.K) {                       // (the columns of a part of a tile are fetched as they are put)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) __builtin_memcpy(&staged[c], src[c] + (size_t)kt * ROW, 16);
+        }
+    };
+    const auto put_x = [&](uint32_t kt, int stage) {
+        if ((kt + 1) * 128 <= g.K) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) R::put(lds + stage * STAGE, dst[c], staged[c]);
+        } else {
+#pragma unroll 1
+            for (int c = 0; c < CH; ++c)
+                R::put(lds + stage * STAGE, R::place(t / CPR + c * (NT / CPR), at), load_end((const X_t*)row_of(c), kt * 128 + at * (I8 ? 16 : 8), g.K));
+        }
+    };
+
+    // ---- W
+    size_t tile_at[TN];
+#pragma unroll
+    for (int c = 0; c < TN; ++c) {
+        const uint32_t nt = n0 / 16 + wn * TN + c;
+        tile_at[c] = (size_t)(nt < g.n_tiles ? nt : g.n_tiles - 1) * g.k_tiles;
+    }
+    uintx4 w[TN];
+    S_t sv[TN];
+    uint32_t zv[TN];
+    const auto fetch_w = [&](uint32_t kt) {
+#pragma unroll
+        for (int c = 0; c < TN; ++c) {
+            const size_t tile = tile_at[c] + kt;
+            w[c] = *(const uintx4*)(g.codes + tile * kQ4TileBytes + lane * 16);
+            sv[c] = *(const S_t*)(g.scales + (tile * 16 + l16) * GPB);
+            zv[c] = 0x08080808u;
+            if constexpr (ZEROS) zv[c] = *(const typename Zeros<GPB>::type*)(g.zeros + (tile * 16 + l16) * GPB);
+        }
+    };
+
+    const WidenF16 widen_f16;
+    const WidenI8<ZEROS> widen_i8;
+    floatx4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int c = 0; c < TN; ++c) acc[i][c] = floatx4{0, 0, 0, 0};
+
+    const uint32_t frag_row = (wm * 16 * TM + l16) * ROW;
+    if (kt0 < kt1) {
+        fetch_x(kt0);
+        fetch_w(kt0);
+        put_x(kt0, 0);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // One group at a time: its codes widened, then (TM tiles of X) x (steps of the group), the fragment of X three steps ahead
+    // on its way from LDS.  The sums of a tile are scaled behind the first product of the next one.  (The barriers to the
+    // scheduler keep the widened codes of other groups, and more fragments than these, out of the registers.)
+    constexpr int XS = I8 && STEPS > 1 ? STEPS / 2 : STEPS, ALL = TM * XS, AHEAD = 3;    // products a tile and group, in all, fragments ahead
+    for (uint32_t kt = kt0; kt < kt1; ++kt) {
+        const unsigned char* from = lds + ((kt - kt0) & 1) * STAGE + frag_row;
+        const bool more = kt + 1 < kt1;
+        if (more) fetch_x(kt + 1);
+        uintx4 wc[TN];
+        S_t sc[TN];
+        uint32_t zc[TN];
+#pragma unroll
+        for (int c = 0; c < TN; ++c) { wc[c] = w[c]; sc[c] = sv[c]; zc[c] = zv[c]; }
+        if (GPB > 1 && more) fetch_w(kt + 1);
+        static_for<0, GPB>([&](auto qc) {
+            constexpr int q = decltype(qc)::value;
+            float s[TN];
+            halfx8 wf[I8 ? 1 : TN][STEPS];
+            uintx2 wi[I8 ? TN : 1][STEPS];
+#pragma unroll
+            for (int c = 0; c < TN; ++c) {
+                if constexpr (GPB == 1) s[c] = (float)sc[c]; else s[c] = (float)sc[c][q];
+                s[c] *= Factor<I8, ZEROS>::value;
+                if (kt * 128 + q * GROUP >= g.K) s[c] = 0.f;         // a group beyond the last column
+                const uint32_t zero = (zc[c] >> (8 * q)) & 0xffu;
+#pragma unroll
+                for (int j = 0; j < STEPS; ++j) {
+                    if constexpr (I8) wi[c][j] = widen_i8(wc[c][q * STEPS + j], zero * 0x01010101u);
+                    else wf[c][j] = widen_f16(wc[c][q * STEPS + j], WidenF16::zero(zero));
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (GPB == 1 && more) fetch_w(kt + 1);
+            typedef typename std::conditional<I8, intx4, floatx4>::type P_t;
+            P_t part[2][TN], none = {0, 0, 0, 0};
+            asm volatile("" : "+v"(none));                 // (else every tile's and group's zeros are four registers of their own, kept across the loop)
+            uintx4 x[AHEAD + 1];
+            const auto read_x = [&](auto fc) {
+                constexpr int f = decltype(fc)::value, i = f / XS, j = f % XS;
+                if constexpr (f < ALL) {
+                    constexpr int chunk = I8 ? (STEPS == 1 ? q / 2 : q * XS + j) * 4 : (q * STEPS + j) * 4;
+                    x[f % (AHEAD + 1)] = *(const uintx4*)(from + i * 16 * ROW + R::slot(chunk + kg, l16));
+                }
+            };
+            static_for<0, AHEAD>(read_x);
+            const auto scale = [&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+#pragma unroll
+                for (int c = 0; c < TN; ++c) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][c][e] = __builtin_fmaf((float)part[i & 1][c][e], s[c], acc[i][c][e]);
+                    asm volatile("" : "+v"(acc[i][c]));    // (else these are moved to the loop's end, where acc is next needed, and every part lives until then)
+                }
+            };
+            static_for<0, ALL>([&](auto fc) {
+                constexpr int f = decltype(fc)::value, i = f / XS, j = f % XS;
+                read_x(std::integral_constant<int, f + AHEAD>{});
+                const uintx4 xv = x[f % (AHEAD + 1)];
+#pragma unroll
+                for (int c = 0; c < TN; ++c) {
+                    const P_t old = j == 0 ? none : part[i & 1][c];
+                    if constexpr (!I8) {
+                        part[i & 1][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, xv), wf[c][j], old, 0, 0, 0);
+                    } else if constexpr (STEPS == 1) {
+                        const uintx2 xh = q % 2 ? uintx2{xv[2], xv[3]} : uintx2{xv[0], xv[1]};
+                        part[i & 1][c] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, xh), __builtin_bit_cast(long, wi[c][0]), old, 0, 0, 0);
+                    } else {
+                        const intx4 b = {(int)wi[c][2 * j][0], (int)wi[c][2 * j][1], (int)wi[c][2 * j + 1][0], (int)wi[c][2 * j + 1][1]};
+                        part[i & 1][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(intx4, xv), b, old, 0, 0, 0);
+                    }
+                }
+                if constexpr (j == 0 && i > 0) scale(std::integral_constant<int, i - 1>{});
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            scale(std::integral_constant<int, TM - 1>{});
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        if (more) put_x(kt + 1, (kt + 1 - kt0) & 1);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+
+    // Epilogue: 16 rows at a time through a buffer of the wavefront's own, so that rows are stored 4 columns a lane
+    float* const turn = (float*)lds + wave * (16 * 16 * TN);
+    constexpr int QUADS = 4 * TN, ROWS_AT_ONCE = 64 / QUADS;
+    static_assert(64 % QUADS == 0, "");
+    const uint32_t col = (lane % QUADS) * 4, n = n0 + wn * 16 * TN + col;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int c = 0; c < TN; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) turn[(4 * kg + e) * (16 * TN) + 16 * c + l16] = acc[i][c][e];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int p = 0; p < 16 / ROWS_AT_ONCE; ++p) {
+            const int r = p * ROWS_AT_ONCE + lane / QUADS;
+            const uint32_t m = m0 + wm * 16 * TM + 16 * i + r;
+            const floatx4 v = *(const floatx4*)(turn + r * (16 * TN) + col);
+            if (m < g.M && n < g.N) {
+                if (g.splits > 1) {
+                    float* out = g.partial + ((size_t)z * g.M + m) * g.partial_ld + n;       // (a whole piece: the pitch is a multiple of 4)
+                    *(floatx4*)out = v;
+                } else {
+                    store_y4(g, m, n, v);
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
+
+// The ranges' sums, in their order, and the epilogue.
+__global__ void __launch_bounds__(256) gemm_q4_join_kernel(const GemmQ4Args g)
+{
+    const uint32_t quads = g.partial_ld / 4;
+    const uint64_t all = (uint64_t)quads * g.M;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
+        const uint32_t m = (uint32_t)(i / quads), n = (uint32_t)(i % quads) * 4;
+        const float* from = g.partial + (size_t)m * g.partial_ld + n;
+        const size_t step = (size_t)g.M * g.partial_ld;
+        floatx4 v = *(const floatx4*)from;
+        for (uint32_t z = 1; z < g.splits; ++z) {
+            const floatx4 p = *(const floatx4*)(from + z * step);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += p[e];
+        }
+        store_y4(g, m, n, v);
+    }
+}
+
 namespace {
+
+template <bool I8, int GPB, bool ZEROS, int TM, int T, int WAVES> int launch_rows(const GemmQ4Args& g, hipStream_t stream)
+{
+    hipLaunchKernelGGL((gemm_q4_rows_kernel<I8, GPB, ZEROS, TM, T, WAVES>), dim3((g.n_tiles + T - 1) / T, (g.M + 16 * TM - 1) / (16 * TM)), dim3(WAVES * 64), 0,
+                       stream, g);
+    return (int)hipGetLastError();
+}
+
+template <bool I8, int GPB, bool ZEROS, int TM, int TN, int WM, int WN> int launch_tiles(const GemmQ4Args& args, hipStream_t stream)
+{
+    GemmQ4Args g = args;
+    constexpr uint32_t BM = 16 * TM * WM, BN = 16 * TN * WN;
+    g.tiles_m = (g.M + BM - 1) / BM;
+    g.tiles_n = (g.N + BN - 1) / BN;
+    if (!g.splits) { g.splits = 1; g.split_tiles = g.k_tiles; }
+    hipLaunchKernelGGL((gemm_q4_tiles_kernel<I8, GPB, ZEROS, TM, TN, WM, WN>), dim3(g.tiles_m * g.tiles_n * g.splits), dim3(WM * WN * 64), 0, stream, g);
+    if (g.splits > 1) {
+        const uint64_t want = ((uint64_t)g.partial_ld / 4 * g.M + 255) / 256;
+        hipLaunchKernelGGL(gemm_q4_join_kernel, dim3((unsigned)(want < 2048 ? want : 2048)), dim3(256), 0, stream, g);
+    }
+    return (int)hipGetLastError();
+}
+
+template <bool I8, int GPB, bool ZEROS> int launch_for(const GemmQ4Args& g, hipStream_t stream)
+{
+#ifdef Q4_EXPERIMENT
+    if (const char* e = getenv("Q4_CFG")) {
+        int kind = 0, sp = 1;
+        sscanf(e, "%d,%d", &kind, &sp);
+        GemmQ4Args a = g;
+        if (sp > 1) {
+            a.splits = sp; a.split_tiles = (g.k_tiles + sp - 1) / sp; a.splits = (g.k_tiles + a.split_tiles - 1) / a.split_tiles;
+            a.partial_ld = (g.N + 3) / 4 * 4; a.partial = (float*)g.workspace;
+        }
+        switch (kind) {
+        case 1: return launch_rows<I8, GPB, ZEROS, 4, 2, 8>(g, stream);
+        case 2: return launch_rows<I8, GPB, ZEROS, 4, 1, 8>(g, stream);
+        case 3: return launch_tiles<I8, GPB, ZEROS, 4, 4, 1, 4>(a, stream);
+        case 4: return launch_tiles<I8, GPB, ZEROS, 4, 2, 1, 4>(a, stream);
+        case 5: return launch_tiles<I8, GPB, ZEROS, 2, 2, 2, 2>(a, stream);
+        case 6: return launch_tiles<I8, GPB, ZEROS, 2, 4, 2, 2>(a, stream);
+        case 7: return launch_tiles<I8, GPB, ZEROS, 4, 2, 2, 4>(a, stream);
+        case 8: return launch_tiles<I8, GPB, ZEROS, 2, 4, 2, 4>(a, stream);
+        }
+    }
+#endif
+    const bool narrow = g.n_tiles <= 256;
+    if (g.M <= 16) {
+        if (narrow) return launch_rows<I8, GPB, ZEROS, 1, 1, 16>(g, stream);
+        if (g.n_tiles < 1024) return launch_rows<I8, GPB, ZEROS, 1, 2, 16>(g, stream);
+        return launch_rows<I8, GPB, ZEROS, 1, 2, 8>(g, stream);
+    }
+    if (g.M <= 32) return narrow ? launch_rows<I8, GPB, ZEROS, 2, 1, 8>(g, stream) : launch_rows<I8, GPB, ZEROS, 2, 2, 8>(g, stream);
+    if (g.M <= 64) return narrow ? launch_rows<I8, GPB, ZEROS, 4, 1, 8>(g, stream) : launch_rows<I8, GPB, ZEROS, 4, 2, 8>(g, stream);
+    return launch_tiles<I8, GPB, ZEROS, 4, 4, 1, 4>(g, stream);
+}
 
 template <bool I8, int GPB> int launch_as(const GemmQ4Args& g, hipStream_t stream)
 {
-    constexpr int TM = 1, T = 1, WAVES = 8;
-    // (the grid's second dimension holds 65 535 workgroups: longer ones go in several launches)
-    constexpr uint32_t ROWS = 16 * TM, MOST = 65535;
-    for (uint32_t m0 = 0; m0 < g.M; m0 += MOST * ROWS) {
-        GemmQ4Args a = g;
-        a.X = (const char*)g.X + (size_t)m0 * g.ldx * (I8 ? 1 : 2);
-        if (g.x_scales) a.x_scales = g.x_scales + m0;
-        if (g.C) a.C = (const char*)g.C + (size_t)m0 * g.ldc * (g.y_f32 ? 4 : 2);
-        a.Y = (char*)g.Y + (size_t)m0 * g.ldy * (g.y_f32 ? 4 : 2);
-        a.M = g.M - m0 < MOST * ROWS ? g.M - m0 : MOST * ROWS;
-        hipLaunchKernelGGL((gemm_q4_rows_kernel<I8, GPB, TM, T, WAVES>), dim3((g.n_tiles + T - 1) / T, (a.M + ROWS - 1) / ROWS), dim3(WAVES * 64), 0, stream, a);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return (int)e;
-        if (g.M - m0 <= MOST * ROWS) break;
-    }
-    return 0;
+    return g.zeros ? launch_for<I8, GPB, true>(g, stream) : launch_for<I8, GPB, false>(g, stream);
 }
 
 }  // namespace

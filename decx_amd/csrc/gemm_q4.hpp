@@ -25,7 +25,14 @@ struct GemmQ4Args {
     uint32_t ldx, ldc, ldy;
     float alpha, beta;
     uint32_t y_f32;
-    uint32_t k_tiles, n_tiles;   // tiles along K and N
+    uint32_t k_tiles, n_tiles;   // tiles of W along K and N
+    uint32_t quads_ok;           // 1: C and Y may be read and written 4 elements at a time
+    uint32_t tiles_m, tiles_n;   // block tiles
+    uint32_t splits;             // ranges of K with workgroups of their own, split_tiles tiles of W each (0 or 1: none)
+    uint32_t split_tiles;
+    uint32_t partial_ld;         // their sums: [range][row][partial_ld], a multiple of 4
+    float* partial;
+    void* workspace;
 };
 
 int launch_gemm_q4(bool i8, uint32_t group, const GemmQ4Args& args, hipStream_t stream);
