@@ -1277,10 +1277,10 @@ static int run_gemm_q4(bool i8, const void* X, const float* x_scales, const void
                        const void* C, void* Y, uint32_t M, uint32_t N, uint32_t K, uint32_t group, uint32_t ldx, uint32_t ldc, uint32_t ldy,
                        float alpha, float beta, int y_is_f32, void* workspace, size_t workspace_bytes, void* stream)
 {
-    (void)workspace_bytes;
     const bool empty = M == 0 || N == 0;
     const uintptr_t y_bytes = y_is_f32 ? 4 : 2;
-    if (!q4_shape_ok(N, K, group)) return DECX_HIP_E_INVALID_ARG;
+    // (a launch has fewer than 2^32 threads: 1024 to a row tile of W, 256 to 64 x 128 outputs)
+    if (!q4_shape_ok(N, K, group) || N > (1u << 25) || ((uint64_t)M / 64 + 1) * ((uint64_t)N / 128 + 1) > (1u << 23)) return DECX_HIP_E_INVALID_ARG;
     if (empty) return g_dev.ready ? DECX_HIP_OK : DECX_HIP_E_NOT_INIT;
     if (!Y || ldy < N || !aligned_to(Y, y_bytes) || (C && ((ldc != 0 && ldc < N) || !aligned_to(C, y_bytes))) || M > 0xffffff00u)
         return DECX_HIP_E_INVALID_ARG;
@@ -1296,11 +1296,11 @@ static int run_gemm_q4(bool i8, const void* X, const float* x_scales, const void
     g.ldx = ldx; g.ldc = ldc; g.ldy = ldy;
     g.alpha = alpha; g.beta = beta;
     g.y_f32 = y_is_f32 ? 1 : 0;
-    g.workspace = workspace;
     g.k_tiles = (K + kQ4TileCols - 1) / kQ4TileCols;
     g.n_tiles = (N + kQ4TileRows - 1) / kQ4TileRows;
     g.quads_ok = (ldy % 4 == 0 && aligned_to(Y, 4 * y_bytes) && (!C || (ldc % 4 == 0 && aligned_to(C, 4 * y_bytes)))) ? 1 : 0;
-    return launch_gemm_q4(i8, group, g, as_stream(stream));
+    const bool room = workspace && aligned16(workspace);
+    return launch_gemm_q4(i8, group, g, room ? workspace : nullptr, room ? workspace_bytes : 0, as_stream(stream));
 }
 
 int decx_hip_gemm_q4_f16(const uint16_t* X, const void* codes, const uint16_t* scales, const uint8_t* zeros, const void* C, void* Y,
@@ -1320,8 +1320,8 @@ int decx_hip_gemm_q4_i8(const int8_t* X, const float* x_scales, const void* code
 
 size_t decx_hip_gemm_q4_workspace(int x_is_i8, uint32_t M, uint32_t N, uint32_t K, uint32_t group)
 {
-    (void)x_is_i8; (void)M; (void)N; (void)K; (void)group;
-    return 0;
+    if (M == 0 || N == 0 || K == 0 || !q4_shape_ok(N, K, group)) return 0;
+    return gemm_q4_workspace(x_is_i8 != 0, M, N, K);
 }
 
 static int run_rmsnorm(bool f16, const void* x, const void* residual, const void* weight, void* sum, void* y, float* y_scales, uint32_t rows,

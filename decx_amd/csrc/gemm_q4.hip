@@ -7,11 +7,6 @@
 // multiplied by its scale, in fp32: no product of code and scale is ever rounded to 16 bits.
 #include "gemm_q4.hpp"
 #include "split_k_exchange.hpp"
-#ifdef Q4_EXPERIMENT
-#include <cstdlib>
-#include <cstdio>
-#endif
-
 namespace decx_hip {
 
 namespace {
@@ -381,11 +376,11 @@ gemm_q4_tiles_kernel(const GemmQ4Args g)
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wm = wave / WN, wn = wave % WN;
     uint32_t tile_m, tile_n, z;
     {
-        // every XCD a contiguous range of tiles, walked in groups of 4 tile rows (gemm_common.hpp, block_to_tile)
+        // every XCD a contiguous range of tiles, walked in groups of 8 tile rows (of 4: 4096 x 8192 x 8192 1.3 % slower)
         const uint32_t tiles = g.tiles_m * g.tiles_n;
         z = blockIdx.x / tiles;
         GemmArgs map;
-        map.tiles_m = g.tiles_m; map.tiles_n = g.tiles_n; map.group_m = 0;
+        map.tiles_m = g.tiles_m; map.tiles_n = g.tiles_n; map.group_m = 8;
         block_to_tile(map, blockIdx.x % tiles, tiles, 0, tile_m, tile_n);
     }
     const uint32_t m0 = tile_m * BM, n0 = tile_n * BN;
@@ -608,7 +603,6 @@ template <bool I8, int GPB, bool ZEROS, int TM, int TN, int WM, int WN> int laun
     constexpr uint32_t BM = 16 * TM * WM, BN = 16 * TN * WN;
     g.tiles_m = (g.M + BM - 1) / BM;
     g.tiles_n = (g.N + BN - 1) / BN;
-    if (!g.splits) { g.splits = 1; g.split_tiles = g.k_tiles; }
     hipLaunchKernelGGL((gemm_q4_tiles_kernel<I8, GPB, ZEROS, TM, TN, WM, WN>), dim3(g.tiles_m * g.tiles_n * g.splits), dim3(WM * WN * 64), 0, stream, g);
     if (g.splits > 1) {
         const uint64_t want = ((uint64_t)g.partial_ld / 4 * g.M + 255) / 256;
@@ -617,53 +611,91 @@ template <bool I8, int GPB, bool ZEROS, int TM, int TN, int WM, int WN> int laun
     return (int)hipGetLastError();
 }
 
-template <bool I8, int GPB, bool ZEROS> int launch_for(const GemmQ4Args& g, hipStream_t stream)
+template <bool I8, int GPB, bool ZEROS> int launch_for(const GemmQ4Args& g, const GemmQ4Plan& p, hipStream_t stream)
 {
-#ifdef Q4_EXPERIMENT
-    if (const char* e = getenv("Q4_CFG")) {
-        int kind = 0, sp = 1;
-        sscanf(e, "%d,%d", &kind, &sp);
-        GemmQ4Args a = g;
-        if (sp > 1) {
-            a.splits = sp; a.split_tiles = (g.k_tiles + sp - 1) / sp; a.splits = (g.k_tiles + a.split_tiles - 1) / a.split_tiles;
-            a.partial_ld = (g.N + 3) / 4 * 4; a.partial = (float*)g.workspace;
-        }
-        switch (kind) {
-        case 1: return launch_rows<I8, GPB, ZEROS, 4, 2, 8>(g, stream);
-        case 2: return launch_rows<I8, GPB, ZEROS, 4, 1, 8>(g, stream);
-        case 3: return launch_tiles<I8, GPB, ZEROS, 4, 4, 1, 4>(a, stream);
-        case 4: return launch_tiles<I8, GPB, ZEROS, 4, 2, 1, 4>(a, stream);
-        case 5: return launch_tiles<I8, GPB, ZEROS, 2, 2, 2, 2>(a, stream);
-        case 6: return launch_tiles<I8, GPB, ZEROS, 2, 4, 2, 2>(a, stream);
-        case 7: return launch_tiles<I8, GPB, ZEROS, 4, 2, 2, 4>(a, stream);
-        case 8: return launch_tiles<I8, GPB, ZEROS, 2, 4, 2, 4>(a, stream);
-        }
+    switch (p.kernel) {
+    case Q4_ROWS_16_NARROW: return launch_rows<I8, GPB, ZEROS, 1, 1, 16>(g, stream);
+    case Q4_ROWS_16:        return launch_rows<I8, GPB, ZEROS, 1, 2, 16>(g, stream);
+    case Q4_ROWS_16_WIDE:   return launch_rows<I8, GPB, ZEROS, 1, 2, 8>(g, stream);
+    case Q4_ROWS_32_NARROW: return launch_rows<I8, GPB, ZEROS, 2, 1, 8>(g, stream);
+    case Q4_ROWS_32:        return launch_rows<I8, GPB, ZEROS, 2, 2, 8>(g, stream);
+    case Q4_ROWS_64_NARROW: return launch_rows<I8, GPB, ZEROS, 4, 1, 8>(g, stream);
+    case Q4_ROWS_64:        return launch_rows<I8, GPB, ZEROS, 4, 2, 8>(g, stream);
+    case Q4_TILES_64x128:   return launch_tiles<I8, GPB, ZEROS, 4, 2, 1, 4>(g, stream);
+    default:                return launch_tiles<I8, GPB, ZEROS, 4, 4, 1, 4>(g, stream);
     }
-#endif
-    const bool narrow = g.n_tiles <= 256;
-    if (g.M <= 16) {
-        if (narrow) return launch_rows<I8, GPB, ZEROS, 1, 1, 16>(g, stream);
-        if (g.n_tiles < 1024) return launch_rows<I8, GPB, ZEROS, 1, 2, 16>(g, stream);
-        return launch_rows<I8, GPB, ZEROS, 1, 2, 8>(g, stream);
-    }
-    if (g.M <= 32) return narrow ? launch_rows<I8, GPB, ZEROS, 2, 1, 8>(g, stream) : launch_rows<I8, GPB, ZEROS, 2, 2, 8>(g, stream);
-    if (g.M <= 64) return narrow ? launch_rows<I8, GPB, ZEROS, 4, 1, 8>(g, stream) : launch_rows<I8, GPB, ZEROS, 4, 2, 8>(g, stream);
-    return launch_tiles<I8, GPB, ZEROS, 4, 4, 1, 4>(g, stream);
 }
 
-template <bool I8, int GPB> int launch_as(const GemmQ4Args& g, hipStream_t stream)
+template <bool I8, int GPB> int launch_as(const GemmQ4Args& g, const GemmQ4Plan& p, hipStream_t stream)
 {
-    return g.zeros ? launch_for<I8, GPB, true>(g, stream) : launch_for<I8, GPB, false>(g, stream);
+    return g.zeros ? launch_for<I8, GPB, true>(g, p, stream) : launch_for<I8, GPB, false>(g, p, stream);
 }
 
 }  // namespace
 
-int launch_gemm_q4(bool i8, uint32_t group, const GemmQ4Args& g, hipStream_t stream)
+// Which kernel, and how many ranges K is cut into.
+// Up to 16 rows the codes decide alone.  One row tile of W per workgroup where there are no more than 256 (a workgroup per CU:
+// 1 x 4096 x 16384 8.6 us, with two 11.5), else two, which halves what X costs (8192 x 8192 7.9 us, with one 8.9); 16
+// wavefronts per workgroup while there are few of them (7 x 5003 x 7001 7.9 us, with 8 9.4), 8 from 512 on (1 x 65536 x 8192
+// 59 us, with 16 69).
+// Beyond, by the time that each is expected to take: the figures below, microseconds, from sweeps of 100 to 4096 rows against
+// 1024 to 8192 columns.  A kernel of few rows takes `step` per column tile of a wavefront and round of 256 workgroups; a tiled one
+// `alone` per column tile with one workgroup on a CU, `full` per round of 512 workgroups.  Ranges pay for storing and reading
+// their sums (7 MB/us) and a second launch.  128 x 8192 x 8192 fp16: 64 x 128 tiles on 4 ranges 30.6 us, whole 73, few-rows
+// kernel 39; 100 x 4096 x 4096: 16.3, 40, 11.9; 4096 x 8192 x 8192: 64 x 256 tiles 508, 64 x 128 595.
+GemmQ4Plan plan_gemm_q4(bool i8, uint32_t M, uint32_t N, uint32_t K, size_t workspace_bytes)
 {
+    const uint32_t nt = (N + kQ4TileRows - 1) / kQ4TileRows, kt = (K + kQ4TileCols - 1) / kQ4TileCols;
+    const bool narrow = nt <= 256;
+    if (M <= 16) return {narrow ? Q4_ROWS_16_NARROW : nt < 1024 ? Q4_ROWS_16 : Q4_ROWS_16_WIDE, 1, kt};
+    GemmQ4Plan best = {Q4_TILES_64x256, 1, kt};
+    if (kt == 0) return best;
+    double best_us = 1e30;
+    const auto consider = [&](int kernel, uint32_t splits, uint32_t len, double us) {
+        if (us < best_us) { best_us = us; best = {kernel, splits, len}; }
+    };
+    {
+        const bool half = M <= 32;
+        const uint64_t wgs = (uint64_t)((M + 63) / 64) * (narrow ? nt : (nt + 1) / 2);
+        const double step = half ? (i8 ? 0.7 : 1.1) : (i8 ? 1.5 : 2.1), rounds = wgs <= 256 ? 1.0 : (double)((wgs + 255) / 256);
+        consider(half ? (narrow ? Q4_ROWS_32_NARROW : Q4_ROWS_32) : (narrow ? Q4_ROWS_64_NARROW : Q4_ROWS_64), 1, kt,
+                 rounds * step * (narrow ? 0.67 : 1.0) * ((kt + 7) / 8));
+    }
+    struct Tile { int kernel; uint32_t columns; double alone, full; };
+    const Tile tiles[2] = {{Q4_TILES_64x256, 256, i8 ? 1.35 : 1.63, i8 ? 1.55 : 1.98}, {Q4_TILES_64x128, 128, i8 ? 1.0 : 1.15, i8 ? 0.84 : 1.24}};
+    const size_t sums = (size_t)M * ((N + 3) / 4 * 4) * 4;
+    for (const Tile& t : tiles) {
+        const uint64_t wgs = (uint64_t)((M + 63) / 64) * ((N + t.columns - 1) / t.columns);
+        for (uint32_t want = 1; want <= 8; ++want) {
+            const uint32_t len = (kt + want - 1) / want, splits = len ? (kt + len - 1) / len : 1;
+            if (splits != want || (want > 1 && (len < 2 || splits * sums > workspace_bytes))) continue;
+            const double round = (double)(wgs * splits) / 512.0;
+            double us = len * (wgs * splits <= 256 ? t.alone : round <= 1.0 ? t.alone + (t.full - t.alone) * (2.0 * round - 1.0) : t.full * round);
+            if (splits > 1) us += 2.0 + (double)splits * sums * 2.0 / 7e6;
+            consider(t.kernel, splits, len, us);
+        }
+    }
+    return best;
+}
+
+size_t gemm_q4_workspace(bool i8, uint32_t M, uint32_t N, uint32_t K)
+{
+    const GemmQ4Plan p = plan_gemm_q4(i8, M, N, K, ~(size_t)0);
+    return p.splits > 1 ? (size_t)p.splits * M * ((N + 3) / 4 * 4) * 4 : 0;
+}
+
+int launch_gemm_q4(bool i8, uint32_t group, const GemmQ4Args& args, void* workspace, size_t workspace_bytes, hipStream_t stream)
+{
+    GemmQ4Args g = args;
+    const GemmQ4Plan p = plan_gemm_q4(i8, g.M, g.N, g.K, workspace_bytes);
+    g.splits = p.splits;
+    g.split_tiles = p.split_tiles;
+    g.partial = (float*)workspace;
+    g.partial_ld = (g.N + 3) / 4 * 4;
     switch (group) {
-    case 128: return i8 ? launch_as<true, 1>(g, stream) : launch_as<false, 1>(g, stream);
-    case 64:  return i8 ? launch_as<true, 2>(g, stream) : launch_as<false, 2>(g, stream);
-    default:  return i8 ? launch_as<true, 4>(g, stream) : launch_as<false, 4>(g, stream);
+    case 128: return i8 ? launch_as<true, 1>(g, p, stream) : launch_as<false, 1>(g, p, stream);
+    case 64:  return i8 ? launch_as<true, 2>(g, p, stream) : launch_as<false, 2>(g, p, stream);
+    default:  return i8 ? launch_as<true, 4>(g, p, stream) : launch_as<false, 4>(g, p, stream);
     }
 }
 

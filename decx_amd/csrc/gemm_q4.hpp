@@ -28,14 +28,21 @@ struct GemmQ4Args {
     uint32_t k_tiles, n_tiles;   // tiles of W along K and N
     uint32_t quads_ok;           // 1: C and Y may be read and written 4 elements at a time
     uint32_t tiles_m, tiles_n;   // block tiles
-    uint32_t splits;             // ranges of K with workgroups of their own, split_tiles tiles of W each (0 or 1: none)
+    uint32_t splits;             // ranges of K with workgroups of their own, split_tiles tiles of W each (1: none)
     uint32_t split_tiles;
     uint32_t partial_ld;         // their sums: [range][row][partial_ld], a multiple of 4
     float* partial;
-    void* workspace;
 };
 
-int launch_gemm_q4(bool i8, uint32_t group, const GemmQ4Args& args, hipStream_t stream);
+enum GemmQ4Kernel : int {
+    Q4_ROWS_16_NARROW, Q4_ROWS_16, Q4_ROWS_16_WIDE, Q4_ROWS_32_NARROW, Q4_ROWS_32, Q4_ROWS_64_NARROW, Q4_ROWS_64,
+    Q4_TILES_64x128, Q4_TILES_64x256,
+};
+struct GemmQ4Plan { int kernel; uint32_t splits, split_tiles; };
+GemmQ4Plan plan_gemm_q4(bool i8, uint32_t M, uint32_t N, uint32_t K, size_t workspace_bytes);
+size_t gemm_q4_workspace(bool i8, uint32_t M, uint32_t N, uint32_t K);
+// fills in the fields of a split; the workspace is 16-byte aligned or null with 0 bytes
+int launch_gemm_q4(bool i8, uint32_t group, const GemmQ4Args& args, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 int launch_q4_quantize(bool f16, const void* W, uint32_t N, uint32_t K, uint32_t ldw, uint32_t group, void* codes, void* scales,
                        void* zeros, hipStream_t stream);

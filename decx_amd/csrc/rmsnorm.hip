@@ -201,11 +201,24 @@ template <typename T, bool Q8> void launch_as(const RmsNormArgs& g, hipStream_t 
 
 }  // namespace
 
-int launch_rmsnorm(bool f16, const RmsNormArgs& g, hipStream_t stream)
+int launch_rmsnorm(bool f16, const RmsNormArgs& args, hipStream_t stream)
 {
-    if (f16) { if (g.y_scales) launch_as<_Float16, true>(g, stream); else launch_as<_Float16, false>(g, stream); }
-    else     { if (g.y_scales) launch_as<float, true>(g, stream);    else launch_as<float, false>(g, stream); }
-    return (int)hipGetLastError();
+    constexpr uint32_t MOST = 1u << 21;                    // rows a launch (it has fewer than 2^32 threads)
+    const size_t e = f16 ? 2 : 4;
+    for (uint64_t r0 = 0; r0 < args.rows; r0 += MOST) {
+        RmsNormArgs g = args;
+        g.rows = args.rows - r0 < MOST ? (uint32_t)(args.rows - r0) : MOST;
+        g.x = (const char*)args.x + r0 * args.ldx * e;
+        if (args.residual) g.residual = (const char*)args.residual + r0 * args.ldr * e;
+        if (args.sum) g.sum = (char*)args.sum + r0 * args.lds * e;
+        g.y = (char*)args.y + r0 * args.ldy * (args.y_scales ? 1 : e);
+        if (args.y_scales) g.y_scales = args.y_scales + r0;
+        if (f16) { if (g.y_scales) launch_as<_Float16, true>(g, stream); else launch_as<_Float16, false>(g, stream); }
+        else     { if (g.y_scales) launch_as<float, true>(g, stream);    else launch_as<float, false>(g, stream); }
+        const hipError_t err = hipGetLastError();
+        if (err != hipSuccess) return (int)err;
+    }
+    return 0;
 }
 
 }  // namespace decx_hip
