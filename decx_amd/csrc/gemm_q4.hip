@@ -66,32 +66,6 @@ __device__ __forceinline__ uintx2 order_i8(uintx2 x)
     return uintx2{__builtin_amdgcn_perm(x[1], x[0], 0x05010400u), __builtin_amdgcn_perm(x[1], x[0], 0x07030602u)};
 }
 
-// 16 bytes of a row from column k on, zero from column K on (for the last column tile; K >= 1): the 16 bytes that end at K,
-// shifted down, so that one load does and nothing behind the row is read.
-template <typename T> __device__ __forceinline__ uintx4 load_end(const T* row, uint32_t k, uint32_t K)
-{
-    constexpr uint32_t E = 16 / sizeof(T);
-    uint64_t low = 0, high = 0;
-    if (k < K && K >= E) {
-        const uint32_t first = k + E <= K ? k : K - E, shift = (k - first) * 8 * sizeof(T);
-        uintx4 v;
-        __builtin_memcpy(&v, row + first, 16);
-        low = (uint64_t)v[1] << 32 | v[0];
-        high = (uint64_t)v[3] << 32 | v[2];
-        if (shift >= 64) { low = high >> (shift - 64); high = 0; }
-        else { low = low >> shift | high << 1 << (63 - shift); high >>= shift; }
-    } else if (k < K) {
-#pragma unroll 1
-        for (uint32_t e = 0; k + e < K; ++e) {             // (rows shorter than that)
-            typename std::conditional<sizeof(T) == 1, uint8_t, uint16_t>::type bits;
-            __builtin_memcpy(&bits, row + k + e, sizeof(T));
-            const uint32_t at = e * 8 * sizeof(T);
-            if (at < 64) low |= (uint64_t)bits << at; else high |= (uint64_t)bits << (at - 64);
-        }
-    }
-    return uintx4{(uint32_t)low, (uint32_t)(low >> 32), (uint32_t)high, (uint32_t)(high >> 32)};
-}
-
 template <int GPB> struct Scales { typedef _Float16 type __attribute__((ext_vector_type(GPB))); };
 template <> struct Scales<1> { typedef _Float16 type; };
 template <int GPB> struct Zeros { typedef uint32_t type; };
@@ -213,8 +187,7 @@ gemm_q4_rows_kernel(const GemmQ4Args g)
         }
     };
     const auto turn_rows = [&](uint32_t kt) {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        wavefront_order();
         if ((kt + 1) * kQ4TileCols <= g.K) {
 #pragma unroll
             for (int c = 0; c < CH; ++c) R::put(turn, R::place(turn_row + c * ROWS_AT_ONCE, turn_at), turning[c]);
@@ -225,9 +198,7 @@ gemm_q4_rows_kernel(const GemmQ4Args g)
                     R::put(turn, R::place(turn_row + c * ROWS_AT_ONCE, turn_at),
                            load_end((const X_t*)(turn_src + c * turn_step), kt * kQ4TileCols + turn_at * (16 / sizeof(X_t)), g.K));
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        wavefront_order();
     };
 
     size_t tile_at[T];
@@ -546,9 +517,7 @@ gemm_q4_tiles_kernel(const GemmQ4Args g)
         for (int c = 0; c < TN; ++c)
 #pragma unroll
             for (int e = 0; e < 4; ++e) turn[(4 * kg + e) * (16 * TN) + 16 * c + l16] = acc[i][c][e];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        wavefront_order();
 #pragma unroll
         for (int p = 0; p < 16 / ROWS_AT_ONCE; ++p) {
             const int r = p * ROWS_AT_ONCE + lane / QUADS;
@@ -563,9 +532,7 @@ gemm_q4_tiles_kernel(const GemmQ4Args g)
                 }
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        wavefront_order();
     }
 }
 

@@ -61,4 +61,38 @@ struct RmsNormArgs {
 };
 int launch_rmsnorm(bool f16, const RmsNormArgs& args, hipStream_t stream);
 
+// 16 bytes of a row from column k on, zero from column K on (for the last columns; K >= 1): the 16 bytes that end at K,
+// shifted down, so that one load does and nothing behind the row is read.
+template <typename T> __device__ __forceinline__ uintx4 load_end(const T* row, uint32_t k, uint32_t K)
+{
+    constexpr uint32_t E = 16 / sizeof(T);
+    uint64_t low = 0, high = 0;
+    if (k < K && K >= E) {
+        const uint32_t first = k + E <= K ? k : K - E, shift = (k - first) * 8 * sizeof(T);
+        uintx4 v;
+        __builtin_memcpy(&v, row + first, 16);
+        low = (uint64_t)v[1] << 32 | v[0];
+        high = (uint64_t)v[3] << 32 | v[2];
+        if (shift >= 64) { low = high >> (shift - 64); high = 0; }
+        else { low = low >> shift | high << 1 << (63 - shift); high >>= shift; }
+    } else if (k < K) {
+#pragma unroll 1
+        for (uint32_t e = 0; k + e < K; ++e) {             // (rows shorter than that)
+            typename std::conditional<sizeof(T) == 1, uint8_t, typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type>::type bits;
+            __builtin_memcpy(&bits, row + k + e, sizeof(T));
+            const uint32_t at = e * 8 * sizeof(T);
+            if (at < 64) low |= (uint64_t)bits << at; else high |= (uint64_t)bits << (at - 64);
+        }
+    }
+    return uintx4{(uint32_t)low, (uint32_t)(low >> 32), (uint32_t)high, (uint32_t)(high >> 32)};
+}
+
+// orders a wavefront's accesses to LDS of its own, which no other wavefront waits for
+__device__ __forceinline__ void wavefront_order()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 }  // namespace decx_hip

@@ -5,8 +5,8 @@
 //                         zero = clamp(rint(-lo / scale), 0, 15),  code = clamp(rint(w / scale) + zero, 0, 15)
 //
 // over the group's columns; scale is computed in fp32 and held in fp16, and what follows uses the held one.  Halves round to
-// even, and a quotient next to a half is decided in 64 bits, so that a code never depends on how a quotient was rounded.
-// Bound: HBM (N K elements in, half a byte each out).  A wavefront makes one tile: a lane reads 8 adjacent columns of its row
+// even, and a quotient next to a half is decided exactly, so that a code never depends on how a quotient was rounded.
+// Bound: HBM (N K elements in, half a byte each out), with the vector pipe close behind: about ten instructions a weight.  A wavefront makes one tile: a lane reads 8 adjacent columns of its row
 // four times (a row's 4 lanes cover 64 or 128 bytes in a row), the extremes of a group meet over those 4 lanes, and the tile
 // is stored 16 bytes per lane, 1 KB in a row.
 #include "gemm_q4.hpp"
@@ -15,41 +15,47 @@ namespace decx_hip {
 
 namespace {
 
-typedef halfx8 halfx8_u __attribute__((aligned(2)));
-typedef floatx4 floatx4_u __attribute__((aligned(4)));
+// eight adjacent weights as they lie in memory
+struct EightF32 { floatx4 a, b; };
+template <typename T> struct Eight { typedef halfx8 type; };
+template <> struct Eight<float> { typedef EightF32 type; };
+__device__ __forceinline__ float element(const halfx8& r, int e) { return (float)r[e]; }
+__device__ __forceinline__ float element(const EightF32& r, int e) { return e < 4 ? r.a[e] : r.b[e - 4]; }
 
-__device__ __forceinline__ void load8(const _Float16* p, float (&v)[8])
+// lo and hi (ZEROS only) and the bits of the largest magnitude so far, as fp32
+template <bool ZEROS> __device__ __forceinline__ void extremes(const halfx8& r, float& lo, float& hi, uint32_t& top)
 {
-    const halfx8 h = *(const halfx8_u*)p;
+    // two at a time: magnitudes as whole numbers
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    const uintx4 w = __builtin_bit_cast(uintx4, r);
+    u16x2 m = {0, 0};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)h[e];
-}
-__device__ __forceinline__ void load8(const float* p, float (&v)[8])
-{
-    const floatx4 a = *(const floatx4_u*)p, b = *(const floatx4_u*)(p + 4);
+    for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu));
+    const uint16_t one = m[0] > m[1] ? m[0] : m[1];
+    const uint32_t bits = __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(_Float16, one));      // (NaN stays NaN, infinity infinity)
+    top = bits > top ? bits : top;
+    if (ZEROS) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+        for (int e = 0; e < 8; ++e) { lo = __builtin_fminf(lo, (float)r[e]); hi = __builtin_fmaxf(hi, (float)r[e]); }
+    }
 }
-__device__ __forceinline__ void store8(_Float16* p, const float (&v)[8])
+template <bool ZEROS> __device__ __forceinline__ void extremes(const EightF32& r, float& lo, float& hi, uint32_t& top)
 {
-    halfx8 h;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = (_Float16)v[e];
-    *(halfx8_u*)p = h;
+    for (int e = 0; e < 8; ++e) {
+        const float x = element(r, e);
+        const uint32_t bits = __builtin_bit_cast(uint32_t, x) & 0x7fffffffu;
+        top = bits > top ? bits : top;
+        if (ZEROS) { lo = __builtin_fminf(lo, x); hi = __builtin_fmaxf(hi, x); }
+    }
 }
-__device__ __forceinline__ void store8(float* p, const float (&v)[8])
+// rint(w / s) by comparison with the half s (m + 1/2) next to the quotient, m = floor(v), v the quotient in fp32: the half is
+// exact in fp32 (11 bits times 6, for quotients that a code can hold), so this is too, ties to even included.
+__device__ __forceinline__ float rint_exactly(float w, float s, float v)
 {
-    *(floatx4_u*)p = floatx4{v[0], v[1], v[2], v[3]};
-    *(floatx4_u*)(p + 4) = floatx4{v[4], v[5], v[6], v[7]};
-}
-
-// rint(w / s) for |w / s| of at most a few tens; inverse = 1 / s in fp32.  The fp32 product is off by less than
-// 16 * 2^-22; only a result that close to a half is asked of the division in 64 bits.
-__device__ __forceinline__ float rint_quotient(float w, float s, float inverse)
-{
-    const float v = w * inverse, r = __builtin_rintf(v);
-    if (__builtin_fabsf(__builtin_fabsf(v - r) - 0.5f) < 1e-4f) return (float)__builtin_rint((double)w / (double)s);
-    return r;
+    const float m = __builtin_floorf(v), half = s * (m + 0.5f);
+    const float even = 2.f * __builtin_rintf(0.5f * m + 0.25f);         // of m and m + 1 the even one
+    return w > half ? m + 1.f : (w < half ? m : even);
 }
 
 }  // namespace
@@ -64,18 +70,33 @@ q4_quantize_kernel(const T* __restrict__ W, uint32_t N, uint32_t K, uint32_t ldw
     const uint64_t tile = (uint64_t)blockIdx.x * PACK_WAVES + (threadIdx.x >> 6);
     if (tile >= tiles) return;
     const int lane = threadIdx.x & 63, r = lane & 15, kg = lane >> 4;
-    const uint32_t n = (uint32_t)(tile / k_tiles) * kQ4TileRows + r, k0 = (uint32_t)(tile % k_tiles) * kQ4TileCols + 8 * kg;
-    float v[4][8];
+    // rows of the tile in LDS: 16-byte chunk c of row r in slot c ^ r, so that 16 rows of a chunk cover all banks
+    constexpr int E = 16 / sizeof(T), CPR = kQ4TileCols / E, AT_ONCE = 64 / CPR;
+    __shared__ __attribute__((aligned(1024))) unsigned char all[PACK_WAVES][16 * CPR * 16];
+    unsigned char* const lds = all[threadIdx.x >> 6];
+    const uint32_t row0 = (uint32_t)(tile / k_tiles) * kQ4TileRows, col0 = (uint32_t)(tile % k_tiles) * kQ4TileCols;
+    const int load_row = lane / CPR, chunk = lane % CPR;
+    uintx4 loaded[CPR / 4];
+    if (row0 + 16 <= N && col0 + kQ4TileCols <= K) {
+#pragma unroll
+        for (int c = 0; c < CPR / 4; ++c) __builtin_memcpy(&loaded[c], W + (size_t)(row0 + load_row + c * AT_ONCE) * ldw + col0 + chunk * E, 16);
+    } else {
+#pragma unroll
+        for (int c = 0; c < CPR / 4; ++c) {
+            const uint32_t n = row0 + load_row + c * AT_ONCE;
+            loaded[c] = n < N ? load_end(W + (size_t)n * ldw, col0 + chunk * E, K) : uintx4{0, 0, 0, 0};
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < CPR / 4; ++c) *(uintx4*)(lds + ((load_row + c * AT_ONCE) * CPR + (chunk ^ (load_row + c * AT_ONCE))) * 16) = loaded[c];
+    wavefront_order();
+    typename Eight<T>::type raw[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const uint32_t k = k0 + 32 * j;
-        const T* p = W + (size_t)n * ldw + k;
-        if (n < N && k + 8 <= K) {
-            load8(p, v[j]);
-        } else {
+        uintx4 v[8 / E];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[j][e] = n < N && k + e < K ? (float)p[e] : 0.f;
-        }
+        for (int h = 0; h < 8 / E; ++h) v[h] = *(const uintx4*)(lds + (r * CPR + (((j * 4 + kg) * (8 / E) + h) ^ r)) * 16);
+        raw[j] = __builtin_bit_cast(typename Eight<T>::type, v);
     }
     constexpr int STEPS = 4 / GPB;
     uintx4 out;
@@ -85,21 +106,15 @@ q4_quantize_kernel(const T* __restrict__ W, uint32_t N, uint32_t K, uint32_t ldw
         float lo = 0.f, hi = 0.f;
         uint32_t top = 0;
 #pragma unroll
-        for (int j = q * STEPS; j < (q + 1) * STEPS; ++j)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = v[j][e];
-                lo = x < lo ? x : lo;
-                hi = x > hi ? x : hi;
-                const uint32_t bits = __builtin_bit_cast(uint32_t, x) & 0x7fffffffu;
-                top = bits > top ? bits : top;
-            }
+        for (int j = q * STEPS; j < (q + 1) * STEPS; ++j) extremes<ZEROS>(raw[j], lo, hi, top);
 #pragma unroll
         for (int off = 16; off <= 32; off <<= 1) {
-            const float l = __shfl_xor(lo, off, 64), h = __shfl_xor(hi, off, 64);
+            if (ZEROS) {
+                const float l = __shfl_xor(lo, off, 64), h = __shfl_xor(hi, off, 64);
+                lo = l < lo ? l : lo;
+                hi = h > hi ? h : hi;
+            }
             const uint32_t b = __shfl_xor(top, off, 64);
-            lo = l < lo ? l : lo;
-            hi = h > hi ? h : hi;
             top = b > top ? b : top;
         }
         const bool finite = top < 0x7f800000u;
@@ -111,25 +126,32 @@ q4_quantize_kernel(const T* __restrict__ W, uint32_t N, uint32_t K, uint32_t ldw
         const float inverse = some ? 1.f / s : 0.f;        // (the smallest fp16 is 2^-24: its inverse is finite)
         float z = 8.f;
         if (ZEROS && some) {
-            z = (float)__builtin_rint(-(double)lo / (double)s);
+            z = rint_exactly(-lo, s, -lo * inverse);
             z = z > 15.f ? 15.f : z;
         }
         const float most = 15.f - z, least = -z;
+        const uint32_t eight_z = (uint32_t)(int)z * 0x11111111u;
 #pragma unroll
         for (int j = q * STEPS; j < (q + 1) * STEPS; ++j) {
-            uint32_t word = 0;
+            // v is off by less than 17 * 2^-23; only where that is enough to cross a half is the exact form asked
+            float v[8], c[8], near = 1.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                float c = 0.f;
-                if (some) {
-                    // a weight beyond the clamp's range by more than a step is clamped before it is divided
-                    const float w = v[j][e], far = 17.f * s, in = w > far ? far : (w < -far ? -far : w);
-                    c = rint_quotient(in, s, inverse);
-                    c = c > most ? most : (c < least ? least : c);
-                }
-                word |= (uint32_t)(int)(c + z) << (4 * (e / 2 + 4 * (e % 2)));
+                v[e] = element(raw[j], e) * inverse;
+                c[e] = __builtin_rintf(v[e]);
+                near = __builtin_fminf(near, __builtin_fabsf(__builtin_fabsf(v[e] - c[e]) - 0.5f));
             }
-            out[j] = word;
+            if (near < 4e-6f) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (__builtin_fabsf(v[e]) < 17.f) c[e] = rint_exactly(element(raw[j], e), s, v[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) c[e] = __builtin_amdgcn_fmed3f(c[e], least, most);
+            // the word's nibbles hold columns 0, 2, 4, 6, 1, 3, 5, 7: four to a sum in fp32, which holds them exactly
+            const auto four = [&](int e) { return (int)__builtin_fmaf(c[e + 6], 4096.f, __builtin_fmaf(c[e + 4], 256.f, __builtin_fmaf(c[e + 2], 16.f, c[e]))); };
+            const uint32_t word = (uint32_t)four(0) + ((uint32_t)four(1) << 16) + eight_z;     // (borrows of negative ones are made good by the zero points)
+            out[j] = some ? word : eight_z;
         }
         if (kg == q % 4) {
             const size_t at = (tile * 16 + r) * GPB + q;
@@ -148,24 +170,38 @@ q4_dequantize_kernel(const unsigned char* __restrict__ codes, const _Float16* __
     const uint64_t tile = (uint64_t)blockIdx.x * PACK_WAVES + (threadIdx.x >> 6);
     if (tile >= tiles) return;
     const int lane = threadIdx.x & 63, r = lane & 15, kg = lane >> 4;
-    const uint32_t n = (uint32_t)(tile / k_tiles) * kQ4TileRows + r, k0 = (uint32_t)(tile % k_tiles) * kQ4TileCols + 8 * kg;
-    if (n >= N) return;
+    constexpr int E = 16 / sizeof(T), CPR = kQ4TileCols / E, AT_ONCE = 64 / CPR;
+    __shared__ __attribute__((aligned(1024))) unsigned char all[PACK_WAVES][16 * CPR * 16];
+    unsigned char* const lds = all[threadIdx.x >> 6];
     const uintx4 w = *(const uintx4*)(codes + tile * kQ4TileBytes + lane * 16);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const size_t at = (tile * 16 + r) * GPB + j * GPB / 4;
         const float s = (float)scales[at];
         const int z = zeros ? zeros[at] : 8;
-        const uint32_t k = k0 + 32 * j;
-        float v[8];
+        T v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (float)((int)((w[j] >> (4 * (e / 2 + 4 * (e % 2)))) & 15u) - z) * s;     // 5 bits by 11: exact in fp32
+        for (int e = 0; e < 8; ++e) v[e] = (T)((float)((int)((w[j] >> (4 * (e / 2 + 4 * (e % 2)))) & 15u) - z) * s);     // 5 bits by 11: exact in fp32
+#pragma unroll
+        for (int h = 0; h < 8 / E; ++h) __builtin_memcpy(lds + (r * CPR + (((j * 4 + kg) * (8 / E) + h) ^ r)) * 16, v + h * E, 16);
+    }
+    wavefront_order();
+    const uint32_t row0 = (uint32_t)(tile / k_tiles) * kQ4TileRows, col0 = (uint32_t)(tile % k_tiles) * kQ4TileCols;
+    const int store_row = lane / CPR, chunk = lane % CPR;
+    const uint32_t k = col0 + chunk * E;
+#pragma unroll
+    for (int c = 0; c < CPR / 4; ++c) {
+        const uint32_t n = row0 + store_row + c * AT_ONCE;
+        if (n >= N || k >= K) continue;
+        const uintx4 v = *(const uintx4*)(lds + ((store_row + c * AT_ONCE) * CPR + (chunk ^ (store_row + c * AT_ONCE))) * 16);
         T* p = W + (size_t)n * ldw + k;
-        if (k + 8 <= K) {
-            store8(p, v);
+        if (k + E <= K) {
+            __builtin_memcpy(p, &v, 16);
         } else {
+            T one[E];
+            __builtin_memcpy(one, &v, 16);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) if (k + e < K) p[e] = (T)v[e];
+            for (int e = 0; e < E; ++e) if (k + e < K) p[e] = one[e];
         }
     }
 }

@@ -58,13 +58,13 @@ template <typename T> __device__ __forceinline__ void store_chunk(T* row, uint32
 __device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint64_t max_of(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
-// rint(127 t / top), inverse = 127 / top: the product is off by less than 127 * 2^-21; only a result that close to a half is
-// asked of the division in 64 bits.
-template <typename A> __device__ __forceinline__ int code_of(A t, A top, A inverse)
+// rint(127 t / top) by comparison with the half top (m + 1/2) next to the quotient, m = floor(v), v the quotient in fp32: both
+// products are exact in 64 bits for fp16 rows.
+__device__ __forceinline__ float rint_exactly(double t, double top, float v)
 {
-    const float v = (float)(t * inverse), r = __builtin_rintf(v);
-    if (__builtin_fabsf(__builtin_fabsf(v - r) - 0.5f) < 1e-4f) return (int)__builtin_rint(127.0 * (double)t / (double)top);
-    return (int)r;
+    const float m = __builtin_floorf(v), even = 2.f * __builtin_rintf(0.5f * m + 0.25f);      // of m and m + 1 the even one
+    const double left = 127.0 * t, half = top * (double)(m + 0.5f);
+    return left > half ? m + 1.f : (left < half ? m : even);
 }
 
 }  // namespace
@@ -149,12 +149,22 @@ rmsnorm_kernel(const RmsNormArgs g)
 
     const auto put = [&](uint32_t k, const typename R::vec& h, const typename R::vec& wv) {
         if constexpr (Q8) {
+            // v is off by less than 127 * 2^-22; only where that is enough to cross a half is the exact form asked
             uint32_t word[2] = {0, 0};
+            float v[n], c[n], near = 1.f;
 #pragma unroll
             for (int e = 0; e < n; ++e) {
-                const int code = some ? code_of<wide>((wide)h[e] * (wide)wv[e], most, inverse) : 0;
-                word[e / 4] |= (uint32_t)(code & 0xff) << (8 * (e % 4));
+                v[e] = (float)((wide)h[e] * (wide)wv[e] * inverse);
+                c[e] = __builtin_rintf(v[e]);
+                near = __builtin_fminf(near, __builtin_fabsf(__builtin_fabsf(v[e] - c[e]) - 0.5f));
             }
+            if (near < 4e-5f) {
+#pragma unroll
+                for (int e = 0; e < n; ++e) c[e] = rint_exactly((double)((wide)h[e] * (wide)wv[e]), (double)most, v[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < n; ++e) word[e / 4] |= ((uint32_t)(int)c[e] & 0xffu) << (8 * (e % 4));
+            if (!some) word[0] = word[1] = 0;              // (a row of zeros, or one that meets what is not finite)
             unsigned char* out = (unsigned char*)g.y + r * g.ldy + k;
             if (k + n <= g.cols) {
                 __builtin_memcpy(out, word, n);
@@ -190,9 +200,15 @@ template <typename T, bool Q8> void launch_as(const RmsNormArgs& g, hipStream_t 
         constexpr int NT = decltype(nt)::value, CHUNKS = decltype(per)::value;
         hipLaunchKernelGGL((rmsnorm_kernel<T, Q8, NT, CHUNKS>), dim3(g.rows), dim3(NT), 0, stream, g);
     };
+    // A thread per 16 bytes of an fp16 row while a workgroup has that many (4096 rows of 8192: 46.0 us, with two, four or eight
+    // pieces a thread 48.5, 52.6, 58.5).  fp32 rows cost twice the arithmetic a byte: two pieces (4096 x 4096: 45.4 us, with
+    // one 48.3), four where two would take 1024 threads (777 x 5001: 8.0 us against 9.7).  From 4096 pieces on (64 KB) the row
+    // is read twice: 800 x 40000 fp16 63.7 us, held eight pieces a thread 64.7.
     using std::integral_constant;
     if (chunks <= 64) go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
     else if (chunks <= 256) go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+    else if (sizeof(T) == 4 && chunks <= 1024) go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+    else if (sizeof(T) == 4 && chunks <= 2048) go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
     else if (chunks <= 1024) go(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
     else if (chunks <= 2048) go(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
     else if (chunks <= 4096) go(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
