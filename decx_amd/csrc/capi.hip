@@ -1321,7 +1321,7 @@ int decx_hip_gemm_q4_i8(const int8_t* X, const float* x_scales, const void* code
 size_t decx_hip_gemm_q4_workspace(int x_is_i8, uint32_t M, uint32_t N, uint32_t K, uint32_t group)
 {
     if (M == 0 || N == 0 || K == 0 || !q4_shape_ok(N, K, group)) return 0;
-    return gemm_q4_workspace(x_is_i8 != 0, M, N, K);
+    return gemm_q4_workspace(x_is_i8 != 0, group, M, N, K);
 }
 
 static int run_rmsnorm(bool f16, const void* x, const void* residual, const void* weight, void* sum, void* y, float* y_scales, uint32_t rows,

@@ -330,7 +330,7 @@ gemm_q4_rows_kernel(const GemmQ4Args g)
 // widens them there, once for all its TM tiles of X.
 template <bool I8, int GPB, bool ZEROS, int TM, int TN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64)
-__attribute__((amdgpu_waves_per_eu(TM * TN >= 32 ? 1 : 2)))
+__attribute__((amdgpu_waves_per_eu(TM * TN >= 16 ? 2 : 3)))
 gemm_q4_tiles_kernel(const GemmQ4Args g)
 {
     constexpr int NT = WM * WN * 64, BM = 16 * TM * WM, BN = 16 * TN * WN;
@@ -366,20 +366,23 @@ gemm_q4_tiles_kernel(const GemmQ4Args g)
         const uint32_t m = m0 + t / CPR + c * (NT / CPR);
         return (const unsigned char*)g.X + (size_t)(m < g.M ? m : g.M - 1) * g.ldx * (I8 ? 1 : 2);       // rows behind the last one: never stored
     };
+    // (Nothing is fetched under a condition: registers that a branch may leave as they were are copied every step.  The columns
+    // of a part of a tile are fetched as they are put; what is fetched in their place is another tile's, or with no whole tile
+    // the first codes.)
+    const uint32_t whole = g.K / 128;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        src[c] = row_of(c) + at * 16;
+        src[c] = whole ? row_of(c) + at * 16 : g.codes;
         dst[c] = R::place(t / CPR + c * (NT / CPR), at);
     }
     uintx4 staged[CH];
     const auto fetch_x = [&](uint32_t kt) {
-        if ((kt + 1) * 128 <= g.K) {                       // (the columns of a part of a tile are fetched as they are put)
+        const size_t from = (size_t)(kt < whole ? kt : whole ? whole - 1 : 0) * ROW;
 #pragma unroll
-            for (int c = 0; c < CH; ++c) __builtin_memcpy(&staged[c], src[c] + (size_t)kt * ROW, 16);
-        }
+        for (int c = 0; c < CH; ++c) __builtin_memcpy(&staged[c], src[c] + from, 16);
     };
     const auto put_x = [&](uint32_t kt, int stage) {
-        if ((kt + 1) * 128 <= g.K) {
+        if (kt < whole) {
 #pragma unroll
             for (int c = 0; c < CH; ++c) R::put(lds + stage * STAGE, dst[c], staged[c]);
         } else {
@@ -419,98 +422,105 @@ gemm_q4_tiles_kernel(const GemmQ4Args g)
         for (int c = 0; c < TN; ++c) acc[i][c] = floatx4{0, 0, 0, 0};
 
     const uint32_t frag_row = (wm * 16 * TM + l16) * ROW;
+    // One group at a time: its codes widened, then (TM tiles of X) x (steps of the group), the fragment of X three steps ahead
+    // on its way from LDS.  The sums of a tile are scaled behind the first product of the next one.  (The barriers to the
+    // scheduler keep the widened codes of other groups, and more fragments than these, out of the registers.)
+    typedef typename std::conditional<I8, intx4, floatx4>::type P_t;
+    constexpr int XS = I8 && STEPS > 1 ? STEPS / 2 : STEPS, ALL = TM * XS, AHEAD = 3;    // products a tile and group, in all, fragments ahead
+    halfx8 wf[I8 ? 1 : TN][STEPS];
+    uintx2 wi[I8 ? TN : 1][STEPS];
+    float s[TN];
+    uintx4 wc[TN];
+    S_t sc[TN];
+    uint32_t zc[TN];
+    const auto widen = [&](uint32_t kt, auto qc) __attribute__((always_inline)) {
+        constexpr int q = decltype(qc)::value;
+#pragma unroll
+        for (int c = 0; c < TN; ++c) {
+            if constexpr (GPB == 1) s[c] = (float)sc[c]; else s[c] = (float)sc[c][q];
+            s[c] *= Factor<I8, ZEROS>::value;
+            if (kt * 128 + q * GROUP >= g.K) s[c] = 0.f;             // a group beyond the last column
+            const uint32_t zero = (zc[c] >> (8 * q)) & 0xffu;
+#pragma unroll
+            for (int j = 0; j < STEPS; ++j) {
+                if constexpr (I8) wi[c][j] = widen_i8(wc[c][q * STEPS + j], zero * 0x01010101u);
+                else wf[c][j] = widen_f16(wc[c][q * STEPS + j], WidenF16::zero(zero));
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto multiply = [&](const unsigned char* from, auto qc) __attribute__((always_inline)) {
+        constexpr int q = decltype(qc)::value;
+        P_t part[2][TN], none = {0, 0, 0, 0};
+        asm volatile("" : "+v"(none));                     // (else every tile's and group's zeros are four registers of their own, kept across the loop)
+        uintx4 x[AHEAD + 1];
+        const auto read_x = [&](auto fc) {
+            constexpr int f = decltype(fc)::value, i = f / XS, j = f % XS;
+            if constexpr (f < ALL) {
+                constexpr int chunk = I8 ? (STEPS == 1 ? q / 2 : q * XS + j) * 4 : (q * STEPS + j) * 4;
+                x[f % (AHEAD + 1)] = *(const uintx4*)(from + i * 16 * ROW + R::slot(chunk + kg, l16));
+            }
+        };
+        static_for<0, AHEAD>(read_x);
+        const auto scale = [&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+#pragma unroll
+            for (int c = 0; c < TN; ++c) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][c][e] = __builtin_fmaf((float)part[i & 1][c][e], s[c], acc[i][c][e]);
+                asm volatile("" : "+v"(acc[i][c]));        // (else these are moved to the loop's end, where acc is next needed, and every part lives until then)
+            }
+        };
+        static_for<0, ALL>([&](auto fc) {
+            constexpr int f = decltype(fc)::value, i = f / XS, j = f % XS;
+            read_x(std::integral_constant<int, f + AHEAD>{});
+            const uintx4 xv = x[f % (AHEAD + 1)];
+#pragma unroll
+            for (int c = 0; c < TN; ++c) {
+                const P_t old = j == 0 ? none : part[i & 1][c];
+                if constexpr (!I8) {
+                    part[i & 1][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, xv), wf[c][j], old, 0, 0, 0);
+                } else if constexpr (STEPS == 1) {
+                    const uintx2 xh = q % 2 ? uintx2{xv[2], xv[3]} : uintx2{xv[0], xv[1]};
+                    part[i & 1][c] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, xh), __builtin_bit_cast(long, wi[c][0]), old, 0, 0, 0);
+                } else {
+                    const intx4 b = {(int)wi[c][2 * j][0], (int)wi[c][2 * j][1], (int)wi[c][2 * j + 1][0], (int)wi[c][2 * j + 1][1]};
+                    part[i & 1][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(intx4, xv), b, old, 0, 0, 0);
+                }
+            }
+            if constexpr (j == 0 && i > 0) scale(std::integral_constant<int, i - 1>{});
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        scale(std::integral_constant<int, TM - 1>{});
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto meet = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     if (kt0 < kt1) {
         fetch_x(kt0);
         fetch_w(kt0);
         put_x(kt0, 0);
     }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    // One group at a time: its codes widened, then (TM tiles of X) x (steps of the group), the fragment of X three steps ahead
-    // on its way from LDS.  The sums of a tile are scaled behind the first product of the next one.  (The barriers to the
-    // scheduler keep the widened codes of other groups, and more fragments than these, out of the registers.)
-    constexpr int XS = I8 && STEPS > 1 ? STEPS / 2 : STEPS, ALL = TM * XS, AHEAD = 3;    // products a tile and group, in all, fragments ahead
+    meet();
     for (uint32_t kt = kt0; kt < kt1; ++kt) {
         const unsigned char* from = lds + ((kt - kt0) & 1) * STAGE + frag_row;
         const bool more = kt + 1 < kt1;
-        if (more) fetch_x(kt + 1);
-        uintx4 wc[TN];
-        S_t sc[TN];
-        uint32_t zc[TN];
+        const uint32_t next = more ? kt + 1 : kt;
+        fetch_x(next);
 #pragma unroll
         for (int c = 0; c < TN; ++c) { wc[c] = w[c]; sc[c] = sv[c]; zc[c] = zv[c]; }
-        if (GPB > 1 && more) fetch_w(kt + 1);
+        if (GPB > 1) fetch_w(next);
         static_for<0, GPB>([&](auto qc) {
-            constexpr int q = decltype(qc)::value;
-            float s[TN];
-            halfx8 wf[I8 ? 1 : TN][STEPS];
-            uintx2 wi[I8 ? TN : 1][STEPS];
-#pragma unroll
-            for (int c = 0; c < TN; ++c) {
-                if constexpr (GPB == 1) s[c] = (float)sc[c]; else s[c] = (float)sc[c][q];
-                s[c] *= Factor<I8, ZEROS>::value;
-                if (kt * 128 + q * GROUP >= g.K) s[c] = 0.f;         // a group beyond the last column
-                const uint32_t zero = (zc[c] >> (8 * q)) & 0xffu;
-#pragma unroll
-                for (int j = 0; j < STEPS; ++j) {
-                    if constexpr (I8) wi[c][j] = widen_i8(wc[c][q * STEPS + j], zero * 0x01010101u);
-                    else wf[c][j] = widen_f16(wc[c][q * STEPS + j], WidenF16::zero(zero));
-                }
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            if (GPB == 1 && more) fetch_w(kt + 1);
-            typedef typename std::conditional<I8, intx4, floatx4>::type P_t;
-            P_t part[2][TN], none = {0, 0, 0, 0};
-            asm volatile("" : "+v"(none));                 // (else every tile's and group's zeros are four registers of their own, kept across the loop)
-            uintx4 x[AHEAD + 1];
-            const auto read_x = [&](auto fc) {
-                constexpr int f = decltype(fc)::value, i = f / XS, j = f % XS;
-                if constexpr (f < ALL) {
-                    constexpr int chunk = I8 ? (STEPS == 1 ? q / 2 : q * XS + j) * 4 : (q * STEPS + j) * 4;
-                    x[f % (AHEAD + 1)] = *(const uintx4*)(from + i * 16 * ROW + R::slot(chunk + kg, l16));
-                }
-            };
-            static_for<0, AHEAD>(read_x);
-            const auto scale = [&](auto ic) {
-                constexpr int i = decltype(ic)::value;
-#pragma unroll
-                for (int c = 0; c < TN; ++c) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][c][e] = __builtin_fmaf((float)part[i & 1][c][e], s[c], acc[i][c][e]);
-                    asm volatile("" : "+v"(acc[i][c]));    // (else these are moved to the loop's end, where acc is next needed, and every part lives until then)
-                }
-            };
-            static_for<0, ALL>([&](auto fc) {
-                constexpr int f = decltype(fc)::value, i = f / XS, j = f % XS;
-                read_x(std::integral_constant<int, f + AHEAD>{});
-                const uintx4 xv = x[f % (AHEAD + 1)];
-#pragma unroll
-                for (int c = 0; c < TN; ++c) {
-                    const P_t old = j == 0 ? none : part[i & 1][c];
-                    if constexpr (!I8) {
-                        part[i & 1][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, xv), wf[c][j], old, 0, 0, 0);
-                    } else if constexpr (STEPS == 1) {
-                        const uintx2 xh = q % 2 ? uintx2{xv[2], xv[3]} : uintx2{xv[0], xv[1]};
-                        part[i & 1][c] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, xh), __builtin_bit_cast(long, wi[c][0]), old, 0, 0, 0);
-                    } else {
-                        const intx4 b = {(int)wi[c][2 * j][0], (int)wi[c][2 * j][1], (int)wi[c][2 * j + 1][0], (int)wi[c][2 * j + 1][1]};
-                        part[i & 1][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(intx4, xv), b, old, 0, 0, 0);
-                    }
-                }
-                if constexpr (j == 0 && i > 0) scale(std::integral_constant<int, i - 1>{});
-                __builtin_amdgcn_sched_barrier(0);
-            });
-            scale(std::integral_constant<int, TM - 1>{});
-            __builtin_amdgcn_sched_barrier(0);
+            widen(kt, qc);
+            if (GPB == 1) fetch_w(next);
+            multiply(from, qc);
         });
         if (more) put_x(kt + 1, (kt + 1 - kt0) & 1);
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        meet();
     }
 
     // Epilogue: 16 rows at a time through a buffer of the wavefront's own, so that rows are stored 4 columns a lane
     float* const turn = (float*)lds + wave * (16 * 16 * TN);
-    constexpr int QUADS = 4 * TN, ROWS_AT_ONCE = 64 / QUADS;
-    static_assert(64 % QUADS == 0, "");
-    const uint32_t col = (lane % QUADS) * 4, n = n0 + wn * 16 * TN + col;
+    constexpr int QUADS = 4 * TN;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -519,9 +529,9 @@ gemm_q4_tiles_kernel(const GemmQ4Args g)
             for (int e = 0; e < 4; ++e) turn[(4 * kg + e) * (16 * TN) + 16 * c + l16] = acc[i][c][e];
         wavefront_order();
 #pragma unroll
-        for (int p = 0; p < 16 / ROWS_AT_ONCE; ++p) {
-            const int r = p * ROWS_AT_ONCE + lane / QUADS;
-            const uint32_t m = m0 + wm * 16 * TM + 16 * i + r;
+        for (int p = 0; p < TN; ++p) {
+            const int r = (p * 64 + lane) / QUADS;
+            const uint32_t col = (p * 64 + lane) % QUADS * 4, m = m0 + wm * 16 * TM + 16 * i + r, n = n0 + wn * 16 * TN + col;
             const floatx4 v = *(const floatx4*)(turn + r * (16 * TN) + col);
             if (m < g.M && n < g.N) {
                 if (g.splits > 1) {
@@ -589,7 +599,8 @@ template <bool I8, int GPB, bool ZEROS> int launch_for(const GemmQ4Args& g, cons
     case Q4_ROWS_64_NARROW: return launch_rows<I8, GPB, ZEROS, 4, 1, 8>(g, stream);
     case Q4_ROWS_64:        return launch_rows<I8, GPB, ZEROS, 4, 2, 8>(g, stream);
     case Q4_TILES_64x128:   return launch_tiles<I8, GPB, ZEROS, 4, 2, 1, 4>(g, stream);
-    default:                return launch_tiles<I8, GPB, ZEROS, 4, 4, 1, 4>(g, stream);
+    case Q4_TILES_64x256:   return launch_tiles<I8, GPB, ZEROS, 4, 4, 1, 4>(g, stream);
+    default:                return launch_tiles<I8, GPB, ZEROS, 8, 3, 1, 8>(g, stream);
     }
 }
 
@@ -606,11 +617,12 @@ template <bool I8, int GPB> int launch_as(const GemmQ4Args& g, const GemmQ4Plan&
 // wavefronts per workgroup while there are few of them (7 x 5003 x 7001 7.9 us, with 8 9.4), 8 from 512 on (1 x 65536 x 8192
 // 59 us, with 16 69).
 // Beyond, by the time that each is expected to take: the figures below, microseconds, from sweeps of 100 to 4096 rows against
-// 1024 to 8192 columns.  A kernel of few rows takes `step` per column tile of a wavefront and round of 256 workgroups; a tiled one
-// `alone` per column tile with one workgroup on a CU, `full` per round of 512 workgroups.  Ranges pay for storing and reading
-// their sums (7 MB/us) and a second launch.  128 x 8192 x 8192 fp16: 64 x 128 tiles on 4 ranges 30.6 us, whole 73, few-rows
-// kernel 39; 100 x 4096 x 4096: 16.3, 40, 11.9; 4096 x 8192 x 8192: 64 x 256 tiles 508, 64 x 128 595.
-GemmQ4Plan plan_gemm_q4(bool i8, uint32_t M, uint32_t N, uint32_t K, size_t workspace_bytes)
+// 1024 to 11000 columns.  A kernel of few rows takes `step` per column tile of a wavefront and round of 256 workgroups; a tiled
+// one `alone` per column tile with one workgroup on a CU, `full` with as many as it holds.  Ranges pay for storing and reading
+// their sums (7 MB/us) and a second launch; groups smaller than 128 for more sums to scale.  fp16: 128 x 8192 x 8192 on tiles of
+// 64 x 128 in 4 ranges 28.8 us, whole 55, few-rows kernel 39.6; 100 x 4096 x 4096: 14.0, 29.6, 11.9; 2048 x 4096 x 4096: 64 x 256
+// tiles 70.8 us, 64 x 128 81, 128 x 384 82; 4096 x 8192 x 8192: 521, 574, 503 (int8 356, 380, 329).
+GemmQ4Plan plan_gemm_q4(bool i8, uint32_t group, uint32_t M, uint32_t N, uint32_t K, size_t workspace_bytes)
 {
     const uint32_t nt = (N + kQ4TileRows - 1) / kQ4TileRows, kt = (K + kQ4TileCols - 1) / kQ4TileCols;
     const bool narrow = nt <= 256;
@@ -626,18 +638,25 @@ GemmQ4Plan plan_gemm_q4(bool i8, uint32_t M, uint32_t N, uint32_t K, size_t work
         const uint64_t wgs = (uint64_t)((M + 63) / 64) * (narrow ? nt : (nt + 1) / 2);
         const double step = half ? (i8 ? 0.7 : 1.1) : (i8 ? 1.5 : 2.1), rounds = wgs <= 256 ? 1.0 : (double)((wgs + 255) / 256);
         consider(half ? (narrow ? Q4_ROWS_32_NARROW : Q4_ROWS_32) : (narrow ? Q4_ROWS_64_NARROW : Q4_ROWS_64), 1, kt,
-                 rounds * step * (narrow ? 0.67 : 1.0) * ((kt + 7) / 8));
+                 rounds * step * (narrow ? 0.67 : 1.0) * ((kt + 7) / 8) * (group == 32 ? 1.2 : 1.0));
     }
-    struct Tile { int kernel; uint32_t columns; double alone, full; };
-    const Tile tiles[2] = {{Q4_TILES_64x256, 256, i8 ? 1.35 : 1.63, i8 ? 1.55 : 1.98}, {Q4_TILES_64x128, 128, i8 ? 1.0 : 1.15, i8 ? 0.84 : 1.24}};
+    struct Tile { int kernel; uint32_t rows, columns, per_cu; double alone, full; };
+    const Tile tiles[3] = {{Q4_TILES_128x384, 128, 384, 1, i8 ? 1.65 : 2.4, i8 ? 1.71 : 2.6}, {Q4_TILES_64x256, 64, 256, 2, i8 ? 1.05 : 1.34, i8 ? 1.39 : 2.03},
+                           {Q4_TILES_64x128, 64, 128, 2, i8 ? 0.71 : 0.86, i8 ? 0.80 : 1.15}};
+    const double finer = group == 128 ? 1.0 : group == 64 ? (i8 ? 1.25 : 1.13) : (i8 ? 1.6 : 1.41);
     const size_t sums = (size_t)M * ((N + 3) / 4 * 4) * 4;
     for (const Tile& t : tiles) {
-        const uint64_t wgs = (uint64_t)((M + 63) / 64) * ((N + t.columns - 1) / t.columns);
+        const uint64_t wgs = (uint64_t)((M + t.rows - 1) / t.rows) * ((N + t.columns - 1) / t.columns);
         for (uint32_t want = 1; want <= 8; ++want) {
             const uint32_t len = (kt + want - 1) / want, splits = len ? (kt + len - 1) / len : 1;
             if (splits != want || (want > 1 && (len < 2 || splits * sums > workspace_bytes))) continue;
-            const double round = (double)(wgs * splits) / 512.0;
-            double us = len * (wgs * splits <= 256 ? t.alone : round <= 1.0 ? t.alone + (t.full - t.alone) * (2.0 * round - 1.0) : t.full * round);
+            // one workgroup a CU: whole rounds; two: they drift apart, and a part of a round is a part of the time
+            const uint64_t all = wgs * splits;
+            const double round = (double)all / 512.0;
+            double us = len * finer;
+            if (all <= 256) us *= t.alone;
+            else if (t.per_cu == 1) us *= t.full * (double)((all + 255) / 256);
+            else us *= round <= 1.0 ? t.alone + (t.full - t.alone) * (2.0 * round - 1.0) : t.full * round;
             if (splits > 1) us += 2.0 + (double)splits * sums * 2.0 / 7e6;
             consider(t.kernel, splits, len, us);
         }
@@ -645,16 +664,16 @@ GemmQ4Plan plan_gemm_q4(bool i8, uint32_t M, uint32_t N, uint32_t K, size_t work
     return best;
 }
 
-size_t gemm_q4_workspace(bool i8, uint32_t M, uint32_t N, uint32_t K)
+size_t gemm_q4_workspace(bool i8, uint32_t group, uint32_t M, uint32_t N, uint32_t K)
 {
-    const GemmQ4Plan p = plan_gemm_q4(i8, M, N, K, ~(size_t)0);
+    const GemmQ4Plan p = plan_gemm_q4(i8, group, M, N, K, ~(size_t)0);
     return p.splits > 1 ? (size_t)p.splits * M * ((N + 3) / 4 * 4) * 4 : 0;
 }
 
 int launch_gemm_q4(bool i8, uint32_t group, const GemmQ4Args& args, void* workspace, size_t workspace_bytes, hipStream_t stream)
 {
     GemmQ4Args g = args;
-    const GemmQ4Plan p = plan_gemm_q4(i8, g.M, g.N, g.K, workspace_bytes);
+    const GemmQ4Plan p = plan_gemm_q4(i8, group, g.M, g.N, g.K, workspace_bytes);
     g.splits = p.splits;
     g.split_tiles = p.split_tiles;
     g.partial = (float*)workspace;

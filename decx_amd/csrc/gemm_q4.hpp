@@ -36,11 +36,11 @@ struct GemmQ4Args {
 
 enum GemmQ4Kernel : int {
     Q4_ROWS_16_NARROW, Q4_ROWS_16, Q4_ROWS_16_WIDE, Q4_ROWS_32_NARROW, Q4_ROWS_32, Q4_ROWS_64_NARROW, Q4_ROWS_64,
-    Q4_TILES_64x128, Q4_TILES_64x256,
+    Q4_TILES_64x128, Q4_TILES_64x256, Q4_TILES_128x384,
 };
 struct GemmQ4Plan { int kernel; uint32_t splits, split_tiles; };
-GemmQ4Plan plan_gemm_q4(bool i8, uint32_t M, uint32_t N, uint32_t K, size_t workspace_bytes);
-size_t gemm_q4_workspace(bool i8, uint32_t M, uint32_t N, uint32_t K);
+GemmQ4Plan plan_gemm_q4(bool i8, uint32_t group, uint32_t M, uint32_t N, uint32_t K, size_t workspace_bytes);
+size_t gemm_q4_workspace(bool i8, uint32_t group, uint32_t M, uint32_t N, uint32_t K);
 // fills in the fields of a split; the workspace is 16-byte aligned or null with 0 bytes
 int launch_gemm_q4(bool i8, uint32_t group, const GemmQ4Args& args, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
