@@ -68,14 +68,17 @@ def build_host(verbose=False):
 
 
 def build_api_test(verbose=False):
-    """The C++ program the tests drive the public de:: API with (tests/cpp/de_api_test)."""
-    src = os.path.join(ROOT, "tests", "cpp", "de_api_test.cpp")
-    out = os.path.join(ROOT, "tests", "cpp", "de_api_test")
-    _run(["g++", "-O1", "-std=c++17", "-Wall", "-pthread", "-I" + os.path.join(ROOT, "include"), src, "-o", out,
-          "-L" + LIB, "-lDECX_BLAS_HIP", "-ldecx_hip", "-Wl,-rpath," + LIB, "-Wl,-rpath,$ORIGIN/../../decx_amd/lib"])
-    if verbose:
-        print("built", out)
-    return out
+    """The C++ programs the tests drive the public de:: API with (tests/cpp/de_api_test, linear4_test)."""
+    outs = []
+    for name in ("de_api_test", "linear4_test"):
+        src = os.path.join(ROOT, "tests", "cpp", name + ".cpp")
+        out = os.path.join(ROOT, "tests", "cpp", name)
+        _run(["g++", "-O1", "-std=c++17", "-Wall", "-pthread", "-I" + os.path.join(ROOT, "include"), src, "-o", out,
+              "-L" + LIB, "-lDECX_BLAS_HIP", "-ldecx_hip", "-Wl,-rpath," + LIB, "-Wl,-rpath,$ORIGIN/../../decx_amd/lib"])
+        if verbose:
+            print("built", out)
+        outs.append(out)
+    return outs
 
 
 def build_all(verbose=False):

@@ -21,7 +21,8 @@
  *
  * Further down: the vector containers and the vector x matrix forms (de::Vector, de::GPU_Vector,
  * srcs/includes/DECX/classes/Vector.h, GPU_Vector.h, BLAS.h:79-80) and the tensor containers with
- * de::nn::cuda::Conv2D (Tensor.h, GPU_Tensor.h, TensorArray.h, BLAS.h:109-110), which call the same kernels.
+ * de::nn::cuda::Conv2D (Tensor.h, GPU_Tensor.h, TensorArray.h, BLAS.h:109-110), which call the same kernels; and, beyond
+ * the original, linear layers with weights in 4 bits (de::GPU_Matrix4, de::nn::cuda::Linear4, RMSNorm).
  * Not provided here: de::blas::cpu::GEMM (the CPU path is not part of this module).
  */
 #ifndef DECX_AMD_PUBLIC_H_
@@ -408,6 +409,25 @@ _DECX_API_ GPU_TensorArray* CreateGPUTensorArrayPtr();
 _DECX_API_ GPU_TensorArray& CreateGPUTensorArrayRef(const _DATA_TYPES_FLAGS_ _type, const uint width, const uint height, const uint depth, const uint32_t _array_length);
 _DECX_API_ GPU_TensorArray* CreateGPUTensorArrayPtr(const _DATA_TYPES_FLAGS_ _type, const uint width, const uint height, const uint depth, const uint32_t _array_length);
 
+/* ------------------------------------------------------------------ device matrix in 4 bits */
+
+/* Height() rows of Width() weights in 4 bits with a scale (and, if HasZeros(), a zero point) for every Group() columns of a
+ * row; made by nn::cuda::Quantize4 (no counterpart in the original library). */
+class _DECX_API_ GPU_Matrix4 {
+public:
+    GPU_Matrix4() {}
+    virtual uint Width() const = 0;
+    virtual uint Height() const = 0;
+    virtual uint Group() const = 0;
+    virtual bool HasZeros() const = 0;
+    virtual void release() = 0;
+    virtual GPU_Matrix4& SoftCopy(GPU_Matrix4& src) = 0;
+    ~GPU_Matrix4() {}
+};
+
+_DECX_API_ GPU_Matrix4& CreateGPUMatrix4Ref();
+_DECX_API_ GPU_Matrix4* CreateGPUMatrix4Ptr();
+
 /* ------------------------------------------------------------------ transfers */
 
 enum DECX_Memcpy_Flags { DECX_MEMCPY_H2D = 0, DECX_MEMCPY_D2H = 1 };
@@ -460,6 +480,38 @@ namespace cuda {
  * left operand is read straight out of the image (no im2col buffer). */
 _DECX_API_ DH Conv2D(GPU_Tensor& src, GPU_TensorArray& kernel, GPU_Tensor& dst, const Point2D strides = {1, 1},
                      const extend_label extend = _EXTEND_NONE_);
+
+/* ---- a linear layer with weights in 4 bits, and the norm in front of it (no counterpart in the original library).
+ * All return when the result is complete; a call that fails its checks leaves its outputs as they were. */
+
+/* dst <- src (fp32 or fp16, outputs x inputs) in 4 bits: a scale, and with zeros a zero point, for every `group` (32, 64
+ * or 128) columns of a row; decx_hip.h has the formulas (decx_hip_q4_quantize_*). */
+_DECX_API_ DH Quantize4(GPU_Matrix& src, GPU_Matrix4& dst, const uint32_t group = 128, const bool zeros = false);
+/* dst <- the values that src stands for; type: _FP16_ or _FP32_. */
+_DECX_API_ DH Dequantize4(GPU_Matrix4& src, GPU_Matrix& dst, const _DATA_TYPES_FLAGS_ type = _FP16_);
+
+/* dst <- src . weights^T: every row of src (fp16, weights.Width() columns) gives weights.Height() outputs.  _fp16_accu
+ * selects their type as in GEMM: fp32 at level 1, else fp16; sums are fp32 either way.
+ * With src_scales, src holds 8-bit codes (_UINT8_ carrying int8) and row r stands for its codes times src_scales[r] (fp32):
+ * what RMSNorm writes.
+ * With C: dst <- alpha . (src . weights^T) + beta . C; C is fp16 or fp32, of dst's size, or a single row that is added to
+ * every row; dst takes its type and may be the same object.  alpha and beta are fp32 or of C's type. */
+_DECX_API_ DH Linear4(GPU_Matrix& src, GPU_Matrix4& weights, GPU_Matrix& dst, const uint32_t _fp16_accu = Fp16_Accurate_L2);
+_DECX_API_ DH Linear4(GPU_Matrix& src, GPU_Vector& src_scales, GPU_Matrix4& weights, GPU_Matrix& dst,
+                      const uint32_t _fp16_accu = Fp16_Accurate_L2);
+_DECX_API_ DH Linear4(GPU_Matrix& src, GPU_Matrix4& weights, GPU_Matrix& C, GPU_Matrix& dst, const Number alpha, const Number beta);
+_DECX_API_ DH Linear4(GPU_Matrix& src, GPU_Vector& src_scales, GPU_Matrix4& weights, GPU_Matrix& C, GPU_Matrix& dst,
+                      const Number alpha, const Number beta);
+
+/* Row by row: sum <- src + residual, dst <- sum . weight / sqrt(mean(sum^2) + eps) (fp32 or fp16, all of src's type; without
+ * residual the norm of src).  With scales dst becomes 8-bit codes (_UINT8_ carrying int8) and scales one fp32 factor a row
+ * (decx_hip_rmsnorm_*).  sum may be src or residual, and dst of src's type any of the three. */
+_DECX_API_ DH RMSNorm(GPU_Matrix& src, GPU_Vector& weight, GPU_Matrix& dst, const float eps = 1e-5f);
+_DECX_API_ DH RMSNorm(GPU_Matrix& src, GPU_Vector& weight, GPU_Matrix& dst, GPU_Vector& scales, const float eps = 1e-5f);
+_DECX_API_ DH RMSNorm(GPU_Matrix& src, GPU_Matrix& residual, GPU_Vector& weight, GPU_Matrix& sum, GPU_Matrix& dst,
+                      const float eps = 1e-5f);
+_DECX_API_ DH RMSNorm(GPU_Matrix& src, GPU_Matrix& residual, GPU_Vector& weight, GPU_Matrix& sum, GPU_Matrix& dst,
+                      GPU_Vector& scales, const float eps = 1e-5f);
 }  // namespace cuda
 }  // namespace nn
 
