@@ -1206,7 +1206,7 @@ static bool q4_shape_ok(uint32_t N, uint32_t K, uint32_t group)
 {
     if (group != 32 && group != 64 && group != 128) return false;
     const uint64_t tiles = (uint64_t)(N / kQ4TileRows + (N % kQ4TileRows != 0)) * (K / kQ4TileCols + (K % kQ4TileCols != 0));
-    return K <= 0xffffff00u && N <= 0xffffff00u && tiles <= 0x7fffffffu;     // (offsets past the last column, and a grid of tiles)
+    return K <= 0xffffff00u && N <= 0xffffff00u && tiles < (1u << 26);       // (offsets past the last column; a launch of 64 threads a tile has fewer than 2^32)
 }
 static inline bool aligned_to(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 // codes are read 16 bytes at a time, the scales and zero points of a tile's row together
@@ -1284,6 +1284,7 @@ static int run_gemm_q4(bool i8, const void* X, const float* x_scales, const void
     if (empty) return g_dev.ready ? DECX_HIP_OK : DECX_HIP_E_NOT_INIT;
     if (!Y || ldy < N || !aligned_to(Y, y_bytes) || (C && ((ldc != 0 && ldc < N) || !aligned_to(C, y_bytes))) || M > 0xffffff00u)
         return DECX_HIP_E_INVALID_ARG;
+    if (C == Y && ldc != ldy && M > 1) return DECX_HIP_E_INVALID_ARG;         // rows would be written that others still add
     if (K > 0 && (!X || ldx < K || (!i8 && !aligned_to(X, 2)) || !q4_parts_ok(codes, scales, zeros, group))) return DECX_HIP_E_INVALID_ARG;
     if (i8 && (!x_scales || !aligned_to(x_scales, 4))) return DECX_HIP_E_INVALID_ARG;
     if (!g_dev.ready) return DECX_HIP_E_NOT_INIT;
@@ -1332,6 +1333,14 @@ static int run_rmsnorm(bool f16, const void* x, const void* residual, const void
     if (!x || !weight || !y || cols == 0 || cols > 0xffff0000u || rows > 0x7fffffffu || ldx < cols || (residual && ldr < cols) ||
         (sum && lds < cols) || ldy < cols || !(eps >= 0.f) || !aligned_to(x, e) || !aligned_to(residual, e) || !aligned_to(weight, e) ||
         !aligned_to(sum, e) || (!y_scales && !aligned_to(y, e)) || !aligned_to(y_scales, 4))
+        return DECX_HIP_E_INVALID_ARG;
+    // an output in the place of an input: element for element, or not at all
+    const auto apart = [&](const void* out, uint32_t ld_out, const void* in, uint32_t ld_in, bool same_type) {
+        return !out || out != in || (same_type && (ld_out == ld_in || rows == 1));
+    };
+    if (!apart(sum, lds, x, ldx, true) || !apart(sum, lds, residual, ldr, true) || !apart(sum, lds, weight, 0, false) || !apart(y, ldy, x, ldx, !y_scales) ||
+        !apart(y, ldy, residual, ldr, !y_scales) || !apart(y, ldy, sum, lds, !y_scales) || !apart(y, ldy, weight, 0, false) || !apart(y_scales, 0, weight, 0, false) ||
+        !apart(y_scales, 0, y, 0, false) || !apart(y_scales, 0, x, 0, false) || !apart(y_scales, 0, residual, 0, false) || !apart(y_scales, 0, sum, 0, false))
         return DECX_HIP_E_INVALID_ARG;
     if (!g_dev.ready) return DECX_HIP_E_NOT_INIT;
     RmsNormArgs g;

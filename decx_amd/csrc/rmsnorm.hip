@@ -207,10 +207,11 @@ template <typename T, bool Q8> void launch_as(const RmsNormArgs& g, hipStream_t 
     using std::integral_constant;
     if (chunks <= 64) go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
     else if (chunks <= 256) go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-    else if (sizeof(T) == 4 && chunks <= 1024) go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
-    else if (sizeof(T) == 4 && chunks <= 2048) go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
-    else if (chunks <= 1024) go(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
-    else if (chunks <= 2048) go(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+    else if (chunks <= 2048) {
+        constexpr bool F32 = sizeof(T) == 4;
+        if (chunks <= 1024) go(integral_constant<int, F32 ? 512 : 1024>{}, integral_constant<int, F32 ? 2 : 1>{});
+        else go(integral_constant<int, F32 ? 512 : 1024>{}, integral_constant<int, F32 ? 4 : 2>{});
+    }
     else if (chunks <= 4096) go(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
     else go(integral_constant<int, 1024>{}, integral_constant<int, 0>{});
 }

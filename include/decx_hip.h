@@ -336,7 +336,7 @@ DECX_HIP_API int decx_hip_q4_dequantize_f16(const void* codes, const uint16_t* s
  * for a 4-bit W.  M = 1 is the matrix x vector product of a single token, bound by reading the codes; M of thousands runs
  * at the rate of the matrix cores.  X is fp16, or int8 where row m stands for X(m, :) * x_scales[m] (what
  * decx_hip_rmsnorm_* writes).  C and Y are fp16, or both fp32 when y_is_f32 != 0; ldc = 0 adds the one row C to every row
- * of Y (a bias); C may be Y.  Products are of X with the whole number code - zero, summed over a group in fp32 (int8: in
+ * of Y (a bias); C may be Y, at Y's pitch.  N is at most 2^25.  Products are of X with the whole number code - zero, summed over a group in fp32 (int8: in
  * int32, exactly) before the scale meets them; sums are fp32, Y is rounded once.  Bases and pitches of X, C and Y need
  * only be whole elements.  workspace: device memory that lets ranges of K be multiplied by workgroups of their own
  * where the output alone would leave CUs idle; NULL or too small is never an error, the sums then run in one piece.
@@ -359,7 +359,8 @@ DECX_HIP_API int decx_hip_gemm_q4_i8(const int8_t* X, const float* x_scales, con
  * y_scales == NULL: y in the rows' type.  Otherwise y holds int8 codes and y_scales one factor per row:
  *   top = max |h * weight|,  code = rint(127 * h * weight / top),  y_scales = top / (127 sqrt(mean(h^2) + eps)) -- the rows
  * decx_hip_gemm_q4_i8 takes.  A row of zeros has scale 0; one that meets a NaN or an infinity has codes 0 and scale NaN.
- * sum may be x or residual, and y (in the rows' type) any of the three, at the same pitch; other overlaps are not allowed.
+ * sum may be x or residual, and y (in the rows' type) any of the three, at the same pitch; other overlaps are not allowed,
+ * and refused where two pointers are equal.
  * Pitches in elements (of y: in elements of its own type), at least cols; any alignment of whole elements.  Sums of squares
  * are kept in fp32 (fp32 rows: 64 bits).  cols = 0 and a negative eps are refused. */
 DECX_HIP_API int decx_hip_rmsnorm_f16(const uint16_t* x, const uint16_t* residual, const uint16_t* weight, uint16_t* sum,
