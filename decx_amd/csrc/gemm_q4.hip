@@ -154,7 +154,10 @@ template <bool I8> struct XRows {
 // themselves and their sums meet in LDS, in wavefront order.  The codes go straight into the registers the matrix instruction
 // reads, 1 KB of a tile a load, one step ahead of the products.  X comes out of the L2, where every wavefront reads other
 // columns of it.  Read in the instruction's order, 16 rows of 64 bytes a load, it would keep the L1 busy with lines; so a
-// wavefront loads whole rows (4 of 256 bytes at a time) and turns them around in LDS of its own, which nobody waits for.
+// wavefront loads whole rows (4 of 256 bytes at a time) and turns them around in LDS of its own, which nobody waits for
+// (7 x 5003 x 7001 20.6 -> 8.1 us, 32 x 8192 x 8192 18.5 -> 12.1).
+// Bound: the codes' way out of HBM, 1 x 65536 x 8192 in groups of 32 60.5 us = 5.0 TB/s; small ones the launch, 1 x 4096 x 4096
+// 4.9 us; from 32 rows on the L1, through which every workgroup draws all of X (60 x 8192 x 4096 int8 10.3 us).
 template <bool I8, int GPB, bool ZEROS, int TM, int T, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64)
 __attribute__((amdgpu_waves_per_eu(TM == 1 ? 4 : 2)))
@@ -328,6 +331,12 @@ gemm_q4_rows_kernel(const GemmQ4Args g)
 // may be unaligned and int8 can be put into the order of the codes on the way.  The codes need no LDS: a wavefront loads the
 // pieces of its TN row tiles straight into the registers the matrix instruction reads them from, one stage ahead, and
 // widens them there, once for all its TM tiles of X.
+// Bound: the issue port that the vector pipe shares with the matrix pipe.  A SIMD takes a v_mfma of 16 cycles every 8 issue
+// cycles at best and a vector instruction every 4; beside 96 of the former a column tile costs a wavefront of 128 x 48 about 235
+// of the latter (9 a word to widen, 4 a tile and group to scale), 128 x 64 more registers than there are, 64 x 64 365.  So the
+// large tile of 128 x 384 holds 8 wavefronts of 128 x 48: 4096 x 8192 x 8192 fp16 498 us (1105 TFLOP/s; of it 8 % for a last
+// round of three quarters, 7 % power: 460 with zeros in X), int8 329 (1670).  64 x 64 each: 520 and 353.  Holding one of a
+// SIMD's two wavefronts back by half a step, so that one widens while the other multiplies: no gain (498 -> 549, int8 340).
 template <bool I8, int GPB, bool ZEROS, int TM, int TN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64)
 __attribute__((amdgpu_waves_per_eu(TM * TN >= 16 ? 2 : 3)))

