@@ -155,10 +155,12 @@ template <bool I8> struct XRows {
 // reads, 1 KB of a tile a load, one step ahead of the products.  X comes out of the L2, where every wavefront reads other
 // columns of it.  Read in the instruction's order, 16 rows of 64 bytes a load, it would keep the L1 busy with lines; so a
 // wavefront loads whole rows (4 of 256 bytes at a time) and turns them around in LDS of its own, which nobody waits for
-// (7 x 5003 x 7001 20.6 -> 8.1 us, 32 x 8192 x 8192 18.5 -> 12.1).
-// Bound: the codes' way out of HBM, 1 x 65536 x 8192 in groups of 32 60.5 us = 5.0 TB/s; small ones the launch, 1 x 4096 x 4096
-// 4.9 us; from 32 rows on the L1, through which every workgroup draws all of X (60 x 8192 x 4096 int8 10.3 us).
-template <bool I8, int GPB, bool ZEROS, int TM, int T, int WAVES>
+// (7 x 5003 x 7001 20.6 -> 8.1 us, 32 x 8192 x 8192 18.5 -> 12.1).  Loads under no condition took 1 x 65536 x 8192 in groups of 32
+// from 60 to 55 us, 1 x 4096 x 16384 from 8.9 to 7.5, 60 x 8192 x 4096 int8 from 10.2 to 9.2; 17 x 5003 x 7001, where the rows
+// are not aligned and half of the loads have none, costs 13.6 for 13.0.
+// Bound: the codes' way out of HBM, 1 x 65536 x 8192 in groups of 32 55 us = 5.5 TB/s; small ones the launch, 1 x 4096 x 4096
+// 5.0 us; from 32 rows on the L1, through which every workgroup draws all of X (60 x 8192 x 4096 int8 9.2 us).
+template <bool I8, int GPB, bool ZEROS, int TM, int T, int WAVES, int CH>
 __global__ void __launch_bounds__(WAVES * 64)
 __attribute__((amdgpu_waves_per_eu(TM == 1 ? 4 : 2)))
 gemm_q4_rows_kernel(const GemmQ4Args g)
@@ -167,7 +169,9 @@ gemm_q4_rows_kernel(const GemmQ4Args g)
     typedef typename std::conditional<I8, intx4, floatx4>::type P_t;
     typedef typename Scales<GPB>::type S_t;
     typedef XRows<I8> R;
-    constexpr int TURN_BYTES = 16 * TM * R::BYTES, CH = TURN_BYTES / 1024, ROWS_AT_ONCE = 64 / R::CHUNKS;
+    constexpr int TURN_BYTES = CH * 1024, ROWS_AT_ONCE = 64 / R::CHUNKS, ROWS = CH * ROWS_AT_ONCE;
+    constexpr bool AHEAD_ALWAYS = CH <= 8;
+    static_assert(ROWS == 16 * TM || (TM == 1 && ROWS < 16 && (ROWS & (ROWS - 1)) == 0), "rows that are held");
     constexpr int RED_BYTES = WAVES * T * TM * 1024;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[WAVES * TURN_BYTES > RED_BYTES ? WAVES * TURN_BYTES : RED_BYTES];
     float (*const red)[T * TM][4][64] = (float (*)[T * TM][4][64])lds;
@@ -176,20 +180,38 @@ gemm_q4_rows_kernel(const GemmQ4Args g)
     const uint32_t tile0 = blockIdx.x * T, m0 = blockIdx.y * (16 * TM);
 
     unsigned char* const turn = lds + wave * TURN_BYTES;
+    // CH loads of ROWS_AT_ONCE rows each.  They and those of the codes are asked for under no condition: behind a branch the
+    // compiler cannot tell a load's wait from that for the loads behind it.  Lanes without a row repeat the last one, loads
+    // without a row read the first codes, and the last whole column tile is read again where none follows (the columns of a
+    // part of a tile are fetched as they are turned).  64 rows of fp16 have no registers for the addresses: there as it was.
     const int turn_row = lane / R::CHUNKS, turn_at = lane % R::CHUNKS;
-    const unsigned char* const turn_src = (const unsigned char*)g.X + (size_t)(m0 + turn_row < g.M ? m0 + turn_row : 0) * g.ldx * sizeof(X_t);
-    const size_t turn_step = (size_t)ROWS_AT_ONCE * g.ldx * sizeof(X_t);
+    const uint32_t here = g.M - m0 < (uint32_t)ROWS ? g.M - m0 : (uint32_t)ROWS, full = here / ROWS_AT_ONCE, rest = here % ROWS_AT_ONCE;
+    const uint32_t whole = g.K / kQ4TileCols;
+    const auto row_at = [&](uint32_t r) __attribute__((always_inline)) { return (const unsigned char*)g.X + (size_t)(m0 + r) * g.ldx * sizeof(X_t); };
+    const unsigned char* const turn_src = AHEAD_ALWAYS && !whole ? g.codes : row_at((uint32_t)turn_row < here ? turn_row : 0);
+    const unsigned char* const rest_src = whole && rest ? row_at((uint32_t)turn_row < rest ? turn_row : rest - 1) : turn_src;
+    const size_t turn_step = AHEAD_ALWAYS && !whole ? 0 : (size_t)ROWS_AT_ONCE * g.ldx * sizeof(X_t);
     uintx4 turning[CH];
-    const auto fetch_rows = [&](uint32_t kt) {
-        if ((kt + 1) * kQ4TileCols <= g.K) {               // (the columns of a part of a tile are fetched as they are turned)
-            const unsigned char* const src = turn_src + ((size_t)kt * kQ4TileCols * sizeof(X_t) + turn_at * 16);
+    const auto fetch_rows = [&](uint32_t kt) __attribute__((always_inline)) {
+        if constexpr (!AHEAD_ALWAYS) {
+            const unsigned char* const src = turn_src + ((size_t)kt * R::BYTES + turn_at * 16);
+            if ((kt + 1) * kQ4TileCols <= g.K)
 #pragma unroll
-            for (int c = 0; c < CH; ++c)
-                if (m0 + turn_row + c * ROWS_AT_ONCE < g.M)    // (rows behind the last one: whatever LDS holds, they are not stored)
-                    __builtin_memcpy(&turning[c], src + c * turn_step, 16);
+                for (int c = 0; c < CH; ++c)
+                    if ((uint32_t)(turn_row + c * ROWS_AT_ONCE) < here) __builtin_memcpy(&turning[c], src + c * turn_step, 16);
+            return;
+        }
+        const size_t from = (size_t)(kt < whole ? kt : whole ? whole - 1 : 0) * R::BYTES + turn_at * 16;
+#pragma unroll
+        for (uint32_t c = 0; c < (uint32_t)CH; ++c) {
+            const bool last = c == full && rest;
+            const unsigned char* src = g.codes;
+            if (c < full) src = turn_src + (from + c * turn_step);
+            if (last) src = rest_src + (from + c * turn_step);
+            __builtin_memcpy(&turning[c], src, 16);
         }
     };
-    const auto turn_rows = [&](uint32_t kt) {
+    const auto turn_rows = [&](uint32_t kt) __attribute__((always_inline)) {
         wavefront_order();
         if ((kt + 1) * kQ4TileCols <= g.K) {
 #pragma unroll
@@ -199,11 +221,13 @@ gemm_q4_rows_kernel(const GemmQ4Args g)
             for (int c = 0; c < CH; ++c)
                 if (m0 + turn_row + c * ROWS_AT_ONCE < g.M)
                     R::put(turn, R::place(turn_row + c * ROWS_AT_ONCE, turn_at),
-                           load_end((const X_t*)(turn_src + c * turn_step), kt * kQ4TileCols + turn_at * (16 / sizeof(X_t)), g.K));
+                           load_end((const X_t*)(AHEAD_ALWAYS ? row_at(turn_row + c * ROWS_AT_ONCE) : turn_src + c * turn_step),
+                                    kt * kQ4TileCols + turn_at * (16 / sizeof(X_t)), g.K));
         }
         wavefront_order();
     };
 
+    const int held = ROWS < 16 ? l16 & (ROWS - 1) : l16;       // (of fewer rows than 16 the same ones again: they are not stored)
     size_t tile_at[T];
 #pragma unroll
     for (int c = 0; c < T; ++c) tile_at[c] = (size_t)(tile0 + c < g.n_tiles ? tile0 + c : g.n_tiles - 1) * g.k_tiles;
@@ -251,7 +275,7 @@ gemm_q4_rows_kernel(const GemmQ4Args g)
                 uintx4 x[TM];
 #pragma unroll
                 for (int i = 0; i < TM; ++i) {
-                    x[i] = *(const uintx4*)(turn + (16 * i + l16) * R::BYTES + R::slot((I8 ? j / 2 : j) * 4 + kg, l16));
+                    x[i] = *(const uintx4*)(turn + (16 * i + held) * R::BYTES + R::slot((I8 ? j / 2 : j) * 4 + kg, held));
                     if constexpr (I8 && BY == 1 && j % 2) { x[i][0] = x[i][2]; x[i][1] = x[i][3]; }
                 }
 #pragma unroll
@@ -286,12 +310,15 @@ gemm_q4_rows_kernel(const GemmQ4Args g)
         });
     };
 
-    // codes for two steps, taking turns
+    // codes for two steps, taking turns; X is asked for before them, since loads are waited for in their order
     Codes a, b;
     uint32_t kt = wave;
     const auto step = [&](const Codes& now, Codes& next) __attribute__((always_inline)) {
         turn_rows(kt);
-        if (kt + WAVES < g.k_tiles) {
+        if constexpr (AHEAD_ALWAYS) {
+            fetch_rows(kt + WAVES);
+            fetch_codes(next, kt + WAVES < g.k_tiles ? kt + WAVES : kt);
+        } else if (kt + WAVES < g.k_tiles) {
             fetch_codes(next, kt + WAVES);
             fetch_rows(kt + WAVES);
         }
@@ -300,8 +327,9 @@ gemm_q4_rows_kernel(const GemmQ4Args g)
         return kt < g.k_tiles;
     };
     if (kt < g.k_tiles) {
+        if constexpr (AHEAD_ALWAYS) fetch_rows(kt);
         fetch_codes(a, kt);
-        fetch_rows(kt);
+        if constexpr (!AHEAD_ALWAYS) fetch_rows(kt);
         while (step(a, b) && step(b, a)) {}
     }
     __syncthreads();
@@ -391,7 +419,7 @@ gemm_q4_tiles_kernel(const GemmQ4Args g)
         for (int c = 0; c < CH; ++c) __builtin_memcpy(&staged[c], src[c] + from, 16);
     };
     const auto put_x = [&](uint32_t kt, int stage) {
-        if (kt < whole) {
+        if ((kt + 1) * kQ4TileCols <= g.K) {
 #pragma unroll
             for (int c = 0; c < CH; ++c) R::put(lds + stage * STAGE, dst[c], staged[c]);
         } else {
@@ -576,9 +604,9 @@ __global__ void __launch_bounds__(256) gemm_q4_join_kernel(const GemmQ4Args g)
 
 namespace {
 
-template <bool I8, int GPB, bool ZEROS, int TM, int T, int WAVES> int launch_rows(const GemmQ4Args& g, hipStream_t stream)
+template <bool I8, int GPB, bool ZEROS, int TM, int T, int WAVES, int CH = (I8 ? 2 : 4) * TM> int launch_rows(const GemmQ4Args& g, hipStream_t stream)
 {
-    hipLaunchKernelGGL((gemm_q4_rows_kernel<I8, GPB, ZEROS, TM, T, WAVES>), dim3((g.n_tiles + T - 1) / T, (g.M + 16 * TM - 1) / (16 * TM)), dim3(WAVES * 64), 0,
+    hipLaunchKernelGGL((gemm_q4_rows_kernel<I8, GPB, ZEROS, TM, T, WAVES, CH>), dim3((g.n_tiles + T - 1) / T, (g.M + 16 * TM - 1) / (16 * TM)), dim3(WAVES * 64), 0,
                        stream, g);
     return (int)hipGetLastError();
 }
@@ -599,6 +627,21 @@ template <bool I8, int GPB, bool ZEROS, int TM, int TN, int WM, int WN> int laun
 
 template <bool I8, int GPB, bool ZEROS> int launch_for(const GemmQ4Args& g, const GemmQ4Plan& p, hipStream_t stream)
 {
+    if (g.M <= (I8 ? 8 : 4)) {                             // (one load of X: fewer registers, less of the L1; 1 x 4096 x 16384 8.9 -> 7.5)
+        switch (p.kernel) {
+        case Q4_ROWS_16_NARROW: return launch_rows<I8, GPB, ZEROS, 1, 1, 16, 1>(g, stream);
+        case Q4_ROWS_16:        return launch_rows<I8, GPB, ZEROS, 1, 2, 16, 1>(g, stream);
+        default:                return launch_rows<I8, GPB, ZEROS, 1, 2, 8, 1>(g, stream);
+        }
+    }
+    if constexpr (!I8)
+        if (g.M <= 8) {                                    // (two: 7 x 5003 x 7001, whose rows are not aligned, 9.4 us with four, 7.7 so)
+            switch (p.kernel) {
+            case Q4_ROWS_16_NARROW: return launch_rows<I8, GPB, ZEROS, 1, 1, 16, 2>(g, stream);
+            case Q4_ROWS_16:        return launch_rows<I8, GPB, ZEROS, 1, 2, 16, 2>(g, stream);
+            default:                return launch_rows<I8, GPB, ZEROS, 1, 2, 8, 2>(g, stream);
+            }
+        }
     switch (p.kernel) {
     case Q4_ROWS_16_NARROW: return launch_rows<I8, GPB, ZEROS, 1, 1, 16>(g, stream);
     case Q4_ROWS_16:        return launch_rows<I8, GPB, ZEROS, 1, 2, 16>(g, stream);
@@ -622,9 +665,9 @@ template <bool I8, int GPB> int launch_as(const GemmQ4Args& g, const GemmQ4Plan&
 
 // Which kernel, and how many ranges K is cut into.
 // Up to 16 rows the codes decide alone.  One row tile of W per workgroup where there are no more than 256 (a workgroup per CU:
-// 1 x 4096 x 16384 8.6 us, with two 11.5), else two, which halves what X costs (8192 x 8192 7.9 us, with one 8.9); 16
-// wavefronts per workgroup while there are few of them (7 x 5003 x 7001 7.9 us, with 8 9.4), 8 from 512 on (1 x 65536 x 8192
-// 59 us, with 16 69).
+// 1 x 4096 x 16384 7.3 us, with two 9.8), else two, which halves what X costs (16 x 8192 x 8192 9.0 us, with one 11.4); 16
+// wavefronts per workgroup while there are few of them (7 x 5003 x 7001 7.9 us, with 8 9.4), 8 from 256 on (1 x 65536 x 8192
+// 53 us, with 16 61; 1 x 11008 x 4096 int8 6.1, with 16 7.3; 16 x 8192 x 8192 8.4, with 16 9.0).
 // Beyond, by the time that each is expected to take: the figures below, microseconds, from sweeps of 100 to 4096 rows against
 // 1024 to 11000 columns.  A kernel of few rows takes `step` per column tile of a wavefront and round of 256 workgroups; a tiled
 // one `alone` per column tile with one workgroup on a CU, `full` with as many as it holds.  Ranges pay for storing and reading
@@ -635,7 +678,7 @@ GemmQ4Plan plan_gemm_q4(bool i8, uint32_t group, uint32_t M, uint32_t N, uint32_
 {
     const uint32_t nt = (N + kQ4TileRows - 1) / kQ4TileRows, kt = (K + kQ4TileCols - 1) / kQ4TileCols;
     const bool narrow = nt <= 256;
-    if (M <= 16) return {narrow ? Q4_ROWS_16_NARROW : nt < 1024 ? Q4_ROWS_16 : Q4_ROWS_16_WIDE, 1, kt};
+    if (M <= 16) return {narrow ? Q4_ROWS_16_NARROW : nt < 512 ? Q4_ROWS_16 : Q4_ROWS_16_WIDE, 1, kt};
     GemmQ4Plan best = {Q4_TILES_64x256, 1, kt};
     if (kt == 0) return best;
     double best_us = 1e30;

@@ -90,6 +90,16 @@ def test_products_of_layers(hip, M, N, K, group, i8):
     run_product(hip, np.random.default_rng([M, N, K]), M, N, K, group, M % 2 == 0, i8, True, c_rows=1, alpha=2.0, beta=1.0)
 
 
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 6, 7, 8, 9, 11, 12, 13, 16, 17, 19, 21, 31, 33, 37, 41, 47, 63])
+@pytest.mark.parametrize("i8", [False, True])
+def test_products_of_few_rows(hip, M, i8):
+    """Every number of loads of X, with and without a part of one, by K below a column tile, of whole ones and with a rest; one
+    and two row tiles of W a workgroup, and 8 and 16 wavefronts."""
+    rng = np.random.default_rng(M)
+    for N, K, group in ((40, 100, 32), (70, 256, 128), (4100, 700, 64), (8200, 300, 128), (8200, 90, 64)):
+        run_product(hip, rng, M, N, K, group, M % 2 == 0, i8, False, ldx=K + M % 3)
+
+
 @pytest.mark.parametrize("off", [1, 3, 7])
 @pytest.mark.parametrize("M,N,K", [(1, 100, 517), (9, 64, 256), (70, 99, 777), (300, 270, 600)])
 def test_products_at_any_alignment(hip, off, M, N, K):

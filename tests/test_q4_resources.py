@@ -10,7 +10,7 @@ def test_products_with_4_bit_weights(tmp_path):
     r = resource_report("gemm_q4.hip", tmp_path)
     rows = {k: v for k, v in r.items() if "gemm_q4_rows_kernel" in k}
     tiles = {k: v for k, v in r.items() if "gemm_q4_tiles_kernel" in k}
-    assert len(rows) == 12 * 7 and len(tiles) == 12 * 3                       # 2 types of X, 3 groups, with and without zero points
+    assert len(rows) == 6 * (10 + 13) and len(tiles) == 12 * 3                # 2 types of X, 3 groups, with and without zero points
     for k, (waves, scratch) in r.items():
         assert scratch == 0, k
     for k, (waves, _) in rows.items():
