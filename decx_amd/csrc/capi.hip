@@ -1273,20 +1273,27 @@ int decx_hip_q4_dequantize_f16(const void* codes, const uint16_t* scales, const 
     return run_q4_dequantize(true, codes, scales, zeros, W, N, K, ldw, group, stream);
 }
 
+// (a launch has fewer than 2^32 threads: 1024 to a row tile of W, 256 to 64 x 128 outputs)
+static bool q4_product_ok(uint32_t M, uint32_t N, uint32_t K, uint32_t group)
+{
+    return q4_shape_ok(N, K, group) && N <= (1u << 25) && ((uint64_t)M / 64 + 1) * ((uint64_t)N / 128 + 1) <= (1u << 23);
+}
+
 static int run_gemm_q4(bool i8, const void* X, const float* x_scales, const void* codes, const uint16_t* scales, const uint8_t* zeros,
                        const void* C, void* Y, uint32_t M, uint32_t N, uint32_t K, uint32_t group, uint32_t ldx, uint32_t ldc, uint32_t ldy,
-                       float alpha, float beta, int y_is_f32, void* workspace, size_t workspace_bytes, void* stream)
+                       float alpha, float beta, int y_is_f32, void* workspace, size_t workspace_bytes, void* stream, const GemmQ4Plan* forced = nullptr)
 {
     const bool empty = M == 0 || N == 0;
     const uintptr_t y_bytes = y_is_f32 ? 4 : 2;
-    // (a launch has fewer than 2^32 threads: 1024 to a row tile of W, 256 to 64 x 128 outputs)
-    if (!q4_shape_ok(N, K, group) || N > (1u << 25) || ((uint64_t)M / 64 + 1) * ((uint64_t)N / 128 + 1) > (1u << 23)) return DECX_HIP_E_INVALID_ARG;
+    if (!q4_product_ok(M, N, K, group)) return DECX_HIP_E_INVALID_ARG;
     if (empty) return g_dev.ready ? DECX_HIP_OK : DECX_HIP_E_NOT_INIT;
     if (!Y || ldy < N || !aligned_to(Y, y_bytes) || (C && ((ldc != 0 && ldc < N) || !aligned_to(C, y_bytes))) || M > 0xffffff00u)
         return DECX_HIP_E_INVALID_ARG;
     if (C == Y && ldc != ldy && M > 1) return DECX_HIP_E_INVALID_ARG;         // rows would be written that others still add
     if (K > 0 && (!X || ldx < K || (!i8 && !aligned_to(X, 2)) || !q4_parts_ok(codes, scales, zeros, group))) return DECX_HIP_E_INVALID_ARG;
     if (i8 && (!x_scales || !aligned_to(x_scales, 4))) return DECX_HIP_E_INVALID_ARG;
+    const size_t room = workspace && aligned16(workspace) ? workspace_bytes : 0;
+    if (forced && !gemm_q4_plan_ok(*forced, M, N, K, room)) return DECX_HIP_E_INVALID_ARG;
     if (!g_dev.ready) return DECX_HIP_E_NOT_INIT;
     GemmQ4Args g;
     std::memset(&g, 0, sizeof g);
@@ -1300,8 +1307,7 @@ static int run_gemm_q4(bool i8, const void* X, const float* x_scales, const void
     g.k_tiles = (K + kQ4TileCols - 1) / kQ4TileCols;
     g.n_tiles = (N + kQ4TileRows - 1) / kQ4TileRows;
     g.quads_ok = (ldy % 4 == 0 && aligned_to(Y, 4 * y_bytes) && (!C || (ldc % 4 == 0 && aligned_to(C, 4 * y_bytes)))) ? 1 : 0;
-    const bool room = workspace && aligned16(workspace);
-    return launch_gemm_q4(i8, group, g, room ? workspace : nullptr, room ? workspace_bytes : 0, as_stream(stream));
+    return launch_gemm_q4(i8, group, g, forced ? *forced : plan_gemm_q4(i8, group, M, N, K, room), room ? workspace : nullptr, as_stream(stream));
 }
 
 int decx_hip_gemm_q4_f16(const uint16_t* X, const void* codes, const uint16_t* scales, const uint8_t* zeros, const void* C, void* Y,
@@ -1323,6 +1329,25 @@ size_t decx_hip_gemm_q4_workspace(int x_is_i8, uint32_t M, uint32_t N, uint32_t 
 {
     if (M == 0 || N == 0 || K == 0 || !q4_shape_ok(N, K, group)) return 0;
     return gemm_q4_workspace(x_is_i8 != 0, group, M, N, K);
+}
+
+int decx_hip_gemm_q4_plan(int x_is_i8, uint32_t M, uint32_t N, uint32_t K, uint32_t group, size_t workspace_bytes, decx_hip_q4_plan* out)
+{
+    if (!out || M == 0 || N == 0 || !q4_product_ok(M, N, K, group)) return DECX_HIP_E_INVALID_ARG;
+    const GemmQ4Plan p = plan_gemm_q4(x_is_i8 != 0, group, M, N, K, workspace_bytes);
+    std::memset(out, 0, sizeof *out);
+    out->kernel = p.kernel; out->k_splits = p.splits; out->split_tiles = p.split_tiles;
+    return DECX_HIP_OK;
+}
+
+int decx_hip_gemm_q4_forced_plan(const decx_hip_q4_plan* plan, const void* X, const float* x_scales, const void* codes, const uint16_t* scales,
+                                 const uint8_t* zeros, const void* C, void* Y, uint32_t M, uint32_t N, uint32_t K, uint32_t group, uint32_t ldx,
+                                 uint32_t ldc, uint32_t ldy, float alpha, float beta, int y_is_f32, void* workspace, size_t workspace_bytes, void* stream)
+{
+    if (!plan || M == 0 || N == 0) return DECX_HIP_E_INVALID_ARG;
+    const GemmQ4Plan p = {plan->kernel, plan->k_splits, plan->split_tiles};
+    return run_gemm_q4(x_scales != nullptr, X, x_scales, codes, scales, zeros, C, Y, M, N, K, group, ldx, ldc, ldy, alpha, beta, y_is_f32, workspace,
+                       workspace_bytes, stream, &p);
 }
 
 static int run_rmsnorm(bool f16, const void* x, const void* residual, const void* weight, void* sum, void* y, float* y_scales, uint32_t rows,

@@ -722,10 +722,21 @@ size_t gemm_q4_workspace(bool i8, uint32_t group, uint32_t M, uint32_t N, uint32
     return p.splits > 1 ? (size_t)p.splits * M * ((N + 3) / 4 * 4) * 4 : 0;
 }
 
-int launch_gemm_q4(bool i8, uint32_t group, const GemmQ4Args& args, void* workspace, size_t workspace_bytes, hipStream_t stream)
+bool gemm_q4_plan_ok(const GemmQ4Plan& p, uint32_t M, uint32_t N, uint32_t K, size_t workspace_bytes)
+{
+    const uint32_t kt = (K + kQ4TileCols - 1) / kQ4TileCols;
+    if (p.kernel < 0 || p.kernel >= Q4_KERNEL_COUNT || p.splits == 0) return false;
+    if ((M <= 16) != (p.kernel <= Q4_ROWS_16_WIDE)) return false;
+    if (p.kernel < Q4_TILES_64x128 && M > 16 && (M <= 32) != (p.kernel <= Q4_ROWS_32)) return false;
+    if (p.splits == 1) return p.split_tiles == kt;
+    const size_t sums = (size_t)M * ((N + 3) / 4 * 4) * 4;
+    return p.kernel >= Q4_TILES_64x128 && p.splits <= 8 && p.split_tiles >= 2 && (kt + p.split_tiles - 1) / p.split_tiles == p.splits &&
+           p.splits * sums <= workspace_bytes;
+}
+
+int launch_gemm_q4(bool i8, uint32_t group, const GemmQ4Args& args, const GemmQ4Plan& p, void* workspace, hipStream_t stream)
 {
     GemmQ4Args g = args;
-    const GemmQ4Plan p = plan_gemm_q4(i8, group, g.M, g.N, g.K, workspace_bytes);
     g.splits = p.splits;
     g.split_tiles = p.split_tiles;
     g.partial = (float*)workspace;

@@ -36,13 +36,15 @@ struct GemmQ4Args {
 
 enum GemmQ4Kernel : int {
     Q4_ROWS_16_NARROW, Q4_ROWS_16, Q4_ROWS_16_WIDE, Q4_ROWS_32_NARROW, Q4_ROWS_32, Q4_ROWS_64_NARROW, Q4_ROWS_64,
-    Q4_TILES_64x128, Q4_TILES_64x256, Q4_TILES_128x384,
+    Q4_TILES_64x128, Q4_TILES_64x256, Q4_TILES_128x384, Q4_KERNEL_COUNT,
 };
 struct GemmQ4Plan { int kernel; uint32_t splits, split_tiles; };
 GemmQ4Plan plan_gemm_q4(bool i8, uint32_t group, uint32_t M, uint32_t N, uint32_t K, size_t workspace_bytes);
 size_t gemm_q4_workspace(bool i8, uint32_t group, uint32_t M, uint32_t N, uint32_t K);
-// fills in the fields of a split; the workspace is 16-byte aligned or null with 0 bytes
-int launch_gemm_q4(bool i8, uint32_t group, const GemmQ4Args& args, void* workspace, size_t workspace_bytes, hipStream_t stream);
+// whether `plan` is one that plan_gemm_q4 could give for such a product and workspace
+bool gemm_q4_plan_ok(const GemmQ4Plan& plan, uint32_t M, uint32_t N, uint32_t K, size_t workspace_bytes);
+// fills in the fields of a split; the workspace is 16-byte aligned and has room for the plan's sums
+int launch_gemm_q4(bool i8, uint32_t group, const GemmQ4Args& args, const GemmQ4Plan& plan, void* workspace, hipStream_t stream);
 
 int launch_q4_quantize(bool f16, const void* W, uint32_t N, uint32_t K, uint32_t ldw, uint32_t group, void* codes, void* scales,
                        void* zeros, hipStream_t stream);

@@ -30,6 +30,10 @@ class Plan(ctypes.Structure):
                 ("grid", _u32), ("k_splits", _u32), ("whole_tiles", _u32)]
 
 
+class Q4Plan(ctypes.Structure):
+    _fields_ = [("kernel", ctypes.c_int32), ("k_splits", _u32), ("split_tiles", _u32)]
+
+
 # name -> (restype, argtypes): every symbol include/decx_hip.h declares
 SYMBOLS = {
     "decx_hip_init": (_int, [_int]),
@@ -79,6 +83,8 @@ SYMBOLS = {
     "decx_hip_gemm_q4_workspace": (_sz, [_int] + [_u32] * 4),
     "decx_hip_gemm_q4_f16": (_int, [_vp] * 6 + [_u32] * 7 + [_f, _f, _int, _vp, _sz, _vp]),
     "decx_hip_gemm_q4_i8": (_int, [_vp] * 7 + [_u32] * 7 + [_f, _f, _int, _vp, _sz, _vp]),
+    "decx_hip_gemm_q4_plan": (_int, [_int] + [_u32] * 4 + [_sz, ctypes.POINTER(Q4Plan)]),
+    "decx_hip_gemm_q4_forced_plan": (_int, [ctypes.POINTER(Q4Plan)] + [_vp] * 7 + [_u32] * 7 + [_f, _f, _int, _vp, _sz, _vp]),
     "decx_hip_rmsnorm_f16": (_int, [_vp] * 6 + [_u32] * 6 + [_f, _vp]),
     "decx_hip_rmsnorm_f32": (_int, [_vp] * 6 + [_u32] * 6 + [_f, _vp]),
     "decx_hip_gemm_f64": (_int, [_vp] * 4 + [_u32] * 7 + [ctypes.c_double, ctypes.c_double, _vp]),
@@ -317,9 +323,15 @@ def dequantize_q4(Q, W, stream=None):
     check(fn(*Q.parts(), W.ptr, Q.rows, Q.cols, W.pitch, Q.group, stream), "dequantize_q4")
 
 
-def gemm_q4(X, Q, Y, C=None, alpha=1.0, beta=1.0, x_scales=None, workspace=None, stream=None):
+def plan_q4(x_is_i8, M, N, K, group, workspace_bytes=0):
+    p = Q4Plan()
+    check(lib().decx_hip_gemm_q4_plan(1 if x_is_i8 else 0, M, N, K, group, workspace_bytes, ctypes.byref(p)))
+    return p
+
+
+def gemm_q4(X, Q, Y, C=None, alpha=1.0, beta=1.0, x_scales=None, workspace=None, stream=None, plan=None):
     """Y = X . Q^T or fma(C, beta, alpha * X . Q^T) on DeviceMatrix operands; X fp16, or int8 with x_scales (M fp32 values);
-    C of one row is added to every row of Y when Y has more."""
+    C of one row is added to every row of Y when Y has more.  plan: a Q4Plan to run on instead of the planner's."""
     M, N, K = X.rows, Q.rows, Q.cols
     assert X.cols == K and (Y.rows, Y.cols) == (M, N) and Y.dtype in (np.float16, np.float32)
     if C is not None:
@@ -330,9 +342,13 @@ def gemm_q4(X, Q, Y, C=None, alpha=1.0, beta=1.0, x_scales=None, workspace=None,
             1 if Y.dtype == np.float32 else 0, *ws, stream)
     if X.dtype == np.int8:
         assert x_scales is not None and x_scales.dtype == np.float32 and x_scales.rows * x_scales.cols == M
-        rc = lib().decx_hip_gemm_q4_i8(X.ptr, x_scales.ptr, *rest)
     else:
         assert X.dtype == np.float16 and x_scales is None
+    if plan is not None:
+        rc = lib().decx_hip_gemm_q4_forced_plan(ctypes.byref(plan), X.ptr, x_scales.ptr if x_scales is not None else None, *rest)
+    elif X.dtype == np.int8:
+        rc = lib().decx_hip_gemm_q4_i8(X.ptr, x_scales.ptr, *rest)
+    else:
         rc = lib().decx_hip_gemm_q4_f16(X.ptr, *rest)
     check(rc, "gemm_q4")
 

@@ -46,6 +46,29 @@ DECX_HIP_API int decx_hip_gemm_forced_plan(int elem_bytes, const void* A, const 
                                            uint32_t ldd, double alpha, double beta, int tile, uint32_t k_splits,
                                            uint32_t whole_tiles, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Which kernel a product with 4-bit weights runs on: up to 16 rows 0 (one row tile of weights and 16 wavefronts a workgroup),
+ * 1 (two, 16), 2 (two, 8); up to 32 rows 3 (one, 8), 4 (two, 8); from 33 rows on 5 and 6 (64 at a time, one and two row
+ * tiles, 8 wavefronts); from 17 on the tiled kernels 7 (64 x 128 outputs), 8 (64 x 256), 9 (128 x 384). */
+typedef struct decx_hip_q4_plan {
+    int32_t  kernel;
+    uint32_t k_splits;             /* ranges of K; 1: none */
+    uint32_t split_tiles;          /* column tiles of the weights (128 columns each) per range; with one range: all */
+} decx_hip_q4_plan;
+/* The planner's pick for decx_hip_gemm_q4_f16 (x_is_i8 == 0) or _i8 with so many bytes of workspace.  Works without a GPU;
+ * products of no outputs and sizes that those refuse are refused here too. */
+DECX_HIP_API int decx_hip_gemm_q4_plan(int x_is_i8, uint32_t M, uint32_t N, uint32_t K, uint32_t group, size_t workspace_bytes,
+                                       decx_hip_q4_plan* out);
+/* decx_hip_gemm_q4_f16 (x_scales == NULL) or _i8 on a plan of the caller's choosing.  Plans that the planner could not give for
+ * any such rows -- kernels 0..2 for more than 16 rows or others for fewer, 3 and 4 for more than 32 or 5 and 6 for fewer, ranges
+ * on kernels other than the tiled ones, shorter than two column tiles, or without room in the workspace -- return
+ * DECX_HIP_E_INVALID_ARG.  For tests: every kernel can be run at sizes small enough to be checked; the product path never
+ * calls it. */
+DECX_HIP_API int decx_hip_gemm_q4_forced_plan(const decx_hip_q4_plan* plan, const void* X, const float* x_scales, const void* codes,
+                                              const uint16_t* scales, const uint8_t* zeros, const void* C, void* Y, uint32_t M,
+                                              uint32_t N, uint32_t K, uint32_t group, uint32_t ldx, uint32_t ldc, uint32_t ldy,
+                                              float alpha, float beta, int y_is_f32, void* workspace, size_t workspace_bytes,
+                                              void* stream);
+
 /* What the split-K counter windows of the current device have seen so far: out[0] windows handed out, out[1] times
  * the ring wrapped round, out[2] requests refused (the product then ran unsplit), out[3] events recorded (only once
  * launches have come from more than one stream), out[4] counters given to launches recorded into graphs, out[5] the
