@@ -1,5 +1,8 @@
 """Every kernel of the products with 4-bit weights on data, each at sizes with a rest in every direction, whatever the planner
-would take there.  Against the definition in 64 bits, with the bound that oracle/q4_reference.py derives."""
+would take there; products on ranges of K with their workspace, alone, in place, recorded and replayed.  Against the definition
+in 64 bits, with the bound that oracle/q4_reference.py derives."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -105,3 +108,78 @@ def test_kernels_of_few_rows(hip, kernel, M, i8):
     for at, (N, K) in enumerate([(50, 2200), (16, 300), (33, 128), (47, 77)]):
         for group in (32, 64, 128):
             Product(hip, M, N, K, group, at % 2 == 0, i8, c=M if at % 2 else None, ldx=at, off=at % 2).run(kernel, ldy=at)
+
+
+# ---- ranges of K -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kernel,bm,bn", TILED)
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("splits,K", [(2, 3 * 128 + 1), (3, 5 * 128), (4, 8 * 128 - 50), (8, 2000)])
+def test_ranges_of_k(hip, kernel, bm, bn, i8, splits, K):
+    """The last range shorter than the others and not, sums of whole quads and with a rest, every form of the epilogue."""
+    group, with_zeros = {2: 32, 3: 64, 4: 128, 8: 64}[splits], splits % 4 == 0
+    for M, N in ((bm + 2, bn + 4), (bm - 7, bn + 1)):
+        plain = Product(hip, M, N, K, group, with_zeros, i8)
+        assert np.array_equal(plain.run(kernel, splits), plain.run(kernel, splits))            # the same call gives the same bits
+        Product(hip, M, N, K, group, with_zeros, i8, f32=True, c=1, alpha=0.5).run(kernel, splits, ldy=N % 4)
+        Product(hip, M, N, K, group, with_zeros, i8, c=M, alpha=0.5, beta=-1.5, ldc=4 - N % 4, off=N % 2).run(kernel, splits)
+        Product(hip, M, N, K, group, with_zeros, i8, c=M, beta=2.0).run(kernel, splits, in_place=True)
+
+
+SPLIT = [(65, 300, 4100, 128, False), (65, 302, 4100, 64, False), (65, 2052, 2100, 128, True), (65, 2050, 2100, 32, True), (256, 2048, 4096, 32, False)]
+
+
+@pytest.mark.parametrize("M,N,K,group,i8", SPLIT)
+def test_products_that_the_planner_splits(hip, M, N, K, group, i8):
+    for c in (None, 1, M):
+        p = Product(hip, M, N, K, group, c == 1, i8, c=c, alpha=0.5 if c else 1.0)
+        ws = p.room()
+        need = ws.pitch
+        assert need > 0 and hip.plan_q4(i8, M, N, K, group, need).k_splits > 1
+        # room for all, none, and too little of it: fewer ranges or none, never an error
+        for given in (ws, None, hip.DeviceMatrix(1, need - 1, np.uint8), hip.DeviceMatrix(1, 16, np.uint8)):
+            y = p.result(ldy=3)
+            print("product", M, N, K, group, i8, "workspace", given.pitch if given else 0, flush=True)
+            p.into(y, workspace=given)
+            hip.sync()
+            p.check(y)
+    y = p.result()
+    y.upload_raw(p.C)
+    p.into(y, workspace=ws, in_place=True)
+    hip.sync()
+    p.check(y)
+
+
+def test_recorded_products_on_ranges_replay_beside_eager_ones(hip):
+    """Two launches that meet in a workspace: recorded, replayed back to back on one stream (which may share it), and beside
+    eager calls on another stream with a workspace of their own."""
+    rt = ctypes.CDLL("libamdhip64.so.7")
+    vp = ctypes.c_void_p
+    stream, other = hip.Stream(), hip.Stream()
+    products = [Product(hip, M, N, K, group, True, i8) for M, N, K, group, i8 in SPLIT]
+    for p in products:
+        ws = [p.room(), p.room()]
+        assert ws[0] is not None
+        ys = [p.result() for _ in range(3)]
+        graph, run = vp(), vp()
+        p.into(ys[0], workspace=ws[0], stream=stream.handle)
+        stream.sync()
+        want = p.check(ys[0])
+        assert rt.hipStreamBeginCapture(stream.handle, 0) == 0
+        p.into(ys[0], workspace=ws[0], stream=stream.handle)
+        p.into(ys[1], workspace=ws[0], stream=stream.handle)
+        assert rt.hipStreamEndCapture(stream.handle, ctypes.byref(graph)) == 0
+        assert rt.hipGraphInstantiate(ctypes.byref(run), graph, None, None, ctypes.c_size_t(0)) == 0
+        for replay in range(4):
+            for y in ys:
+                y.upload_raw(np.full((y.rows, y.pitch), -3.0, y.dtype))
+            ws[0].upload_raw(np.full((1, ws[0].pitch), 255, np.uint8))        # (NaNs: sums that were not written show)
+            print("replay", p.shape, replay, flush=True)
+            p.into(ys[2], workspace=ws[1], stream=other.handle)
+            assert rt.hipGraphLaunch(run, stream.handle) == 0
+            p.into(ys[2], workspace=ws[1], stream=other.handle)
+            assert rt.hipGraphLaunch(run, stream.handle) == 0
+            stream.sync(); other.sync()
+            assert all(np.array_equal(y.download_raw(), want) for y in ys)
+        assert rt.hipGraphExecDestroy(run) == 0 and rt.hipGraphDestroy(graph) == 0
+    stream.destroy(); other.destroy()
