@@ -1337,6 +1337,8 @@ int decx_hip_gemm_q4_plan(int x_is_i8, uint32_t M, uint32_t N, uint32_t K, uint3
     const GemmQ4Plan p = plan_gemm_q4(x_is_i8 != 0, group, M, N, K, workspace_bytes);
     std::memset(out, 0, sizeof *out);
     out->kernel = p.kernel; out->k_splits = p.splits; out->split_tiles = p.split_tiles;
+    const uint32_t most = gemm_q4_rows_a_launch(p.kernel, M, N);
+    out->launch_rows = M < most ? M : most;
     return DECX_HIP_OK;
 }
 

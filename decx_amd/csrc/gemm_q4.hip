@@ -604,11 +604,30 @@ __global__ void __launch_bounds__(256) gemm_q4_join_kernel(const GemmQ4Args g)
 
 namespace {
 
-template <bool I8, int GPB, bool ZEROS, int TM, int T, int WAVES, int CH = (I8 ? 2 : 4) * TM> int launch_rows(const GemmQ4Args& g, hipStream_t stream)
+// Rows that one launch of a kernel of few rows takes: a grid has at most 65535 workgroups in y, a launch fewer than 2^32 threads.
+// (Outputs of a few columns and millions of rows: 5000000 x 16 x 512 would have 78125.)
+uint32_t rows_a_launch(uint32_t across, uint32_t tm, uint32_t waves)
 {
-    hipLaunchKernelGGL((gemm_q4_rows_kernel<I8, GPB, ZEROS, TM, T, WAVES, CH>), dim3((g.n_tiles + T - 1) / T, (g.M + 16 * TM - 1) / (16 * TM)), dim3(WAVES * 64), 0,
-                       stream, g);
-    return (int)hipGetLastError();
+    const uint32_t by_threads = 0xffffffffu / (waves * 64) / across;
+    return (by_threads < 65535u ? by_threads : 65535u) * 16 * tm;
+}
+
+template <bool I8, int GPB, bool ZEROS, int TM, int T, int WAVES, int CH = (I8 ? 2 : 4) * TM> int launch_rows(const GemmQ4Args& args, hipStream_t stream)
+{
+    const uint32_t across = (args.n_tiles + T - 1) / T, most = rows_a_launch(across, TM, WAVES);
+    const size_t y_bytes = args.y_f32 ? 4 : 2;
+    for (uint64_t m0 = 0; m0 < args.M; m0 += most) {
+        GemmQ4Args g = args;
+        g.M = args.M - m0 < most ? (uint32_t)(args.M - m0) : most;
+        g.X = (const char*)args.X + m0 * args.ldx * (I8 ? 1 : 2);
+        if (args.x_scales) g.x_scales = args.x_scales + m0;
+        if (args.C) g.C = (const char*)args.C + m0 * args.ldc * y_bytes;
+        g.Y = (char*)args.Y + m0 * args.ldy * y_bytes;
+        hipLaunchKernelGGL((gemm_q4_rows_kernel<I8, GPB, ZEROS, TM, T, WAVES, CH>), dim3(across, (g.M + 16 * TM - 1) / (16 * TM)), dim3(WAVES * 64), 0, stream, g);
+        const hipError_t err = hipGetLastError();
+        if (err != hipSuccess) return (int)err;
+    }
+    return 0;
 }
 
 template <bool I8, int GPB, bool ZEROS, int TM, int TN, int WM, int WN> int launch_tiles(const GemmQ4Args& args, hipStream_t stream)
@@ -720,6 +739,14 @@ size_t gemm_q4_workspace(bool i8, uint32_t group, uint32_t M, uint32_t N, uint32
 {
     const GemmQ4Plan p = plan_gemm_q4(i8, group, M, N, K, ~(size_t)0);
     return p.splits > 1 ? (size_t)p.splits * M * ((N + 3) / 4 * 4) * 4 : 0;
+}
+
+uint32_t gemm_q4_rows_a_launch(int kernel, uint32_t M, uint32_t N)
+{
+    const uint32_t nt = (N + kQ4TileRows - 1) / kQ4TileRows;
+    const bool narrow = kernel == Q4_ROWS_16_NARROW || kernel == Q4_ROWS_32_NARROW || kernel == Q4_ROWS_64_NARROW;
+    const uint32_t tm = kernel <= Q4_ROWS_16_WIDE ? 1 : kernel <= Q4_ROWS_32 ? 2 : 4;
+    return kernel >= Q4_TILES_64x128 ? M : rows_a_launch(narrow ? nt : (nt + 1) / 2, tm, kernel <= Q4_ROWS_16 ? 16 : 8);
 }
 
 bool gemm_q4_plan_ok(const GemmQ4Plan& p, uint32_t M, uint32_t N, uint32_t K, size_t workspace_bytes)

@@ -41,6 +41,7 @@ enum GemmQ4Kernel : int {
 struct GemmQ4Plan { int kernel; uint32_t splits, split_tiles; };
 GemmQ4Plan plan_gemm_q4(bool i8, uint32_t group, uint32_t M, uint32_t N, uint32_t K, size_t workspace_bytes);
 size_t gemm_q4_workspace(bool i8, uint32_t group, uint32_t M, uint32_t N, uint32_t K);
+uint32_t gemm_q4_rows_a_launch(int kernel, uint32_t M, uint32_t N);
 // whether `plan` is one that plan_gemm_q4 could give for such a product and workspace
 bool gemm_q4_plan_ok(const GemmQ4Plan& plan, uint32_t M, uint32_t N, uint32_t K, size_t workspace_bytes);
 // fills in the fields of a split; the workspace is 16-byte aligned and has room for the plan's sums

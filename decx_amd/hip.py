@@ -31,7 +31,7 @@ class Plan(ctypes.Structure):
 
 
 class Q4Plan(ctypes.Structure):
-    _fields_ = [("kernel", ctypes.c_int32), ("k_splits", _u32), ("split_tiles", _u32)]
+    _fields_ = [("kernel", ctypes.c_int32), ("k_splits", _u32), ("split_tiles", _u32), ("launch_rows", _u32)]
 
 
 # name -> (restype, argtypes): every symbol include/decx_hip.h declares

@@ -336,7 +336,8 @@ DECX_HIP_API int decx_hip_q4_dequantize_f16(const void* codes, const uint16_t* s
  * for a 4-bit W.  M = 1 is the matrix x vector product of a single token, bound by reading the codes; M of thousands runs
  * at the rate of the matrix cores.  X is fp16, or int8 where row m stands for X(m, :) * x_scales[m] (what
  * decx_hip_rmsnorm_* writes).  C and Y are fp16, or both fp32 when y_is_f32 != 0; ldc = 0 adds the one row C to every row
- * of Y (a bias); C may be Y, at Y's pitch.  N is at most 2^25.  Products are of X with the whole number code - zero, summed over a group in fp32 (int8: in
+ * of Y (a bias); C may be Y, at Y's pitch.  N is at most 2^25, (M / 64 + 1) (N / 128 + 1) (quotients rounded down)
+ * at most 2^23.  Products are of X with the whole number code - zero, summed over a group in fp32 (int8: in
  * int32, exactly) before the scale meets them; sums are fp32, Y is rounded once.  Bases and pitches of X, C and Y need
  * only be whole elements.  workspace: device memory that lets ranges of K be multiplied by workgroups of their own
  * where the output alone would leave CUs idle; NULL or too small is never an error, the sums then run in one piece.

@@ -53,6 +53,7 @@ typedef struct decx_hip_q4_plan {
     int32_t  kernel;
     uint32_t k_splits;             /* ranges of K; 1: none */
     uint32_t split_tiles;          /* column tiles of the weights (128 columns each) per range; with one range: all */
+    uint32_t launch_rows;          /* rows of X that one launch takes, M unless there are millions of them (forced plans: not read) */
 } decx_hip_q4_plan;
 /* The planner's pick for decx_hip_gemm_q4_f16 (x_is_i8 == 0) or _i8 with so many bytes of workspace.  Works without a GPU;
  * products of no outputs and sizes that those refuse are refused here too. */

@@ -110,6 +110,14 @@ def test_kernels_of_few_rows(hip, kernel, M, i8):
             Product(hip, M, N, K, group, at % 2 == 0, i8, c=M if at % 2 else None, ldx=at, off=at % 2).run(kernel, ldy=at)
 
 
+@pytest.mark.parametrize("kernel,i8", [(ROWS_64_NARROW, False), (ROWS_64_NARROW, True), (ROWS_64, True)])
+def test_more_rows_than_a_grid_has_workgroups_for(hip, kernel, i8):
+    """The rows of the second launch: X, its factors, C and Y each from their place on."""
+    M = 65535 * 64 + 70
+    for c in (None, 1, M):
+        Product(hip, M, 2, 3, 128, False, i8, c=c, ldx=1).run(kernel, ldy=1)
+
+
 # ---- ranges of K -----------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("kernel,bm,bn", TILED)

@@ -58,3 +58,17 @@ def test_plans_that_the_planner_could_not_give_are_refused(M, plan):
     for xs in (None, P(32)):
         assert hip.lib().decx_hip_gemm_q4_forced_plan(ctypes.byref(p), P(32), xs, *rest) == BAD
     assert hip.lib().decx_hip_gemm_q4_forced_plan(None, P(32), None, *rest) == BAD
+
+
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("M,N,K", [(5000000, 16, 512), (1 << 28, 16, 300), (1 << 28, 32, 1000), (65535 * 64, 16, 512), (65535 * 64 + 1, 16, 512)])
+def test_many_rows_and_few_columns_fit_their_grid(i8, M, N, K):
+    """64 rows a workgroup in y, of which a grid has at most 65535; fewer than 2^32 threads a launch."""
+    p = hip.plan_q4(i8, M, N, K, 128)
+    if p.kernel in (ROWS_64_NARROW, ROWS_64):
+        assert p.launch_rows == min(M, 65535 * 64)
+        assert 512 * -(-N // 16) * -(-p.launch_rows // 64) < 1 << 32
+    else:
+        assert p.kernel >= TILES_64x128 and p.launch_rows == M
+    assert hip.plan_q4(i8, 5000000, 16, 512, 128).kernel == ROWS_64_NARROW          # (so the first of them is one that the rule is there for)
+    assert hip.plan_q4(i8, 60, 8192, 4096, 128).launch_rows == 60
