@@ -1206,7 +1206,7 @@ static bool q4_shape_ok(uint32_t N, uint32_t K, uint32_t group)
 {
     if (group != 32 && group != 64 && group != 128) return false;
     const uint64_t tiles = (uint64_t)(N / kQ4TileRows + (N % kQ4TileRows != 0)) * (K / kQ4TileCols + (K % kQ4TileCols != 0));
-    return K <= 0xffffff00u && N <= 0xffffff00u && tiles < (1u << 26);       // (offsets past the last column; a launch of 64 threads a tile has fewer than 2^32)
+    return K <= 0xffffff00u && N <= 0xffffff00u && tiles <= (1u << 26) - 4;  // (offsets past the last column; a launch of 256 threads for every 4 tiles has fewer than 2^32)
 }
 static inline bool aligned_to(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 // codes are read 16 bytes at a time, the scales and zero points of a tile's row together
