@@ -6,6 +6,7 @@
 #include "gemm_q4.hpp"
 #include "split_k_exchange.hpp"
 #include "split_counter_ring.hpp"
+#include "operand_overlap.hpp"
 
 #include <chrono>
 #include <cstring>
@@ -1236,6 +1237,7 @@ static int run_q4_quantize(bool f16, const void* W, void* codes, uint16_t* scale
         return DECX_HIP_E_INVALID_ARG;
     if (!g_dev.ready) return DECX_HIP_E_NOT_INIT;
     if (empty) return DECX_HIP_OK;
+    if (!quantize_operands_apart(W, codes, scales, zeros)) return DECX_HIP_E_INVALID_ARG;
     return launch_q4_quantize(f16, W, N, K, ldw, group, codes, scales, zeros, as_stream(stream));
 }
 
@@ -1259,6 +1261,7 @@ static int run_q4_dequantize(bool f16, const void* codes, const uint16_t* scales
         return DECX_HIP_E_INVALID_ARG;
     if (!g_dev.ready) return DECX_HIP_E_NOT_INIT;
     if (empty) return DECX_HIP_OK;
+    if (!dequantize_operands_apart(W, codes, scales, zeros)) return DECX_HIP_E_INVALID_ARG;
     return launch_q4_dequantize(f16, codes, scales, zeros, W, N, K, ldw, group, as_stream(stream));
 }
 
@@ -1295,6 +1298,8 @@ static int run_gemm_q4(bool i8, const void* X, const float* x_scales, const void
     const size_t room = workspace && aligned16(workspace) ? workspace_bytes : 0;
     if (forced && !gemm_q4_plan_ok(*forced, M, N, K, room)) return DECX_HIP_E_INVALID_ARG;
     if (!g_dev.ready) return DECX_HIP_E_NOT_INIT;
+    if (!product_operands_apart(K ? X : nullptr, x_scales, K ? codes : nullptr, K ? scales : nullptr, K ? zeros : nullptr, C, Y, room ? workspace : nullptr))
+        return DECX_HIP_E_INVALID_ARG;
     GemmQ4Args g;
     std::memset(&g, 0, sizeof g);
     g.X = X; g.x_scales = x_scales;

@@ -320,7 +320,8 @@ DECX_HIP_API size_t decx_hip_q4_scales_count(uint32_t N, uint32_t K, uint32_t gr
  *                   code = clamp(rint(w / scale) + zero, 0, 15)
  * with the scale computed in fp32, at most 65504, and rounded to fp16, the rounded one being divided by; halves round to
  * even and no quotient's rounding decides a code.  A group whose scale rounds to zero holds code = zero = 8; one that
- * holds a NaN or an infinity gets scale NaN. */
+ * holds a NaN or an infinity gets scale NaN.  W and the three arrays lie apart (equal pointers are refused, here and on the
+ * way back). */
 DECX_HIP_API int decx_hip_q4_quantize_f32(const float* W, void* codes, uint16_t* scales, uint8_t* zeros, uint32_t N, uint32_t K,
                                           uint32_t ldw, uint32_t group, void* stream);
 DECX_HIP_API int decx_hip_q4_quantize_f16(const uint16_t* W, void* codes, uint16_t* scales, uint8_t* zeros, uint32_t N, uint32_t K,
@@ -336,7 +337,8 @@ DECX_HIP_API int decx_hip_q4_dequantize_f16(const void* codes, const uint16_t* s
  * for a 4-bit W.  M = 1 is the matrix x vector product of a single token, bound by reading the codes; M of thousands runs
  * at the rate of the matrix cores.  X is fp16, or int8 where row m stands for X(m, :) * x_scales[m] (what
  * decx_hip_rmsnorm_* writes).  C and Y are fp16, or both fp32 when y_is_f32 != 0; ldc = 0 adds the one row C to every row
- * of Y (a bias); C may be Y, at Y's pitch.  N is at most 2^25, (M / 64 + 1) (N / 128 + 1) (quotients rounded down)
+ * of Y (a bias); C may be Y, at Y's pitch; apart from that neither Y nor the workspace may overlap
+ * another operand, and equal pointers are refused.  N is at most 2^25, (M / 64 + 1) (N / 128 + 1) (quotients rounded down)
  * at most 2^23.  Products are of X with the whole number code - zero, summed over a group in fp32 (int8: in
  * int32, exactly) before the scale meets them; sums are fp32, Y is rounded once.  Bases and pitches of X, C and Y need
  * only be whole elements.  workspace: device memory that lets ranges of K be multiplied by workgroups of their own

@@ -1,13 +1,16 @@
 """Calls of the 4-bit layer that are refused, and their neighbours that are not (no GPU: refusals come before the library looks
 for one, and the others end with "not initialised" in a process of their own)."""
 import ctypes
+import os
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 
 from decx_amd import hip
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 P, BAD, NOT_INIT = ctypes.c_void_p, -1, -2
 
 
@@ -35,3 +38,47 @@ def test_more_tiles_than_a_launch_has_threads_for(name, N, K):
 
 def test_the_largest_number_of_tiles():
     calls_get_as_far_as_the_missing_gpu("for name in t.QUANTISE: assert t.quantise(name, 960, 1118481 * 128) == t.NOT_INIT\n")
+
+
+def test_rules_about_operands_in_one_place(tmp_path):
+    exe = str(tmp_path / "operand_overlap_test")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Wextra", "-Werror", os.path.join(ROOT, "tests", "cpp", "operand_overlap_test.cpp"), "-o", exe],
+                   check=True, timeout=300)
+    run = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0 and "all ok" in run.stdout, run.stdout + run.stderr
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i8", [False, True])
+def test_operands_in_one_place_are_refused(i8):
+    """Through the entry points (the rules are asked only once the library is initialised); every buffer is large enough for
+    whatever the call says it is, and a refused call leaves it as it was."""
+    hip.init()
+    L = hip.lib()
+    M, N, K = 20, 64, 128
+    names = ["X", "xs", "codes", "scales", "zeros", "C", "Y", "ws"]
+    at = {n: hip.DeviceMatrix(1, 1 << 17, np.uint8, data=np.full((1, 1 << 17), 5, np.uint8)) for n in names + ["W"]}
+
+    def product(**place):
+        p = {n: at[place.get(n, n)].ptr for n in names}
+        rest = (p["codes"], p["scales"], p["zeros"], p["C"], p["Y"], M, N, K, 64, K, N, N, 1.0, 1.0, 0, p["ws"], 1 << 17, None)
+        return L.decx_hip_gemm_q4_i8(p["X"], p["xs"], *rest) if i8 else L.decx_hip_gemm_q4_f16(p["X"], *rest)
+
+    def quantise(there, **place):
+        p = {n: at[place.get(n, n)].ptr for n in ("W", "codes", "scales", "zeros")}
+        parts = (p["codes"], p["scales"], p["zeros"])
+        if there:
+            return L.decx_hip_q4_quantize_f16(p["W"], *parts, N, K, K, 64, None)
+        return L.decx_hip_q4_dequantize_f16(*parts, p["W"], N, K, K, 64, None)
+    for other in ("X", "codes", "scales", "zeros") + (("xs",) if i8 else ()):
+        assert product(Y=other) == BAD and product(ws=other) == BAD, other
+    assert product(ws="C") == BAD and product(ws="Y") == BAD
+    for a, b in (("W", "codes"), ("W", "scales"), ("W", "zeros")):
+        assert quantise(True, **{a: b}) == BAD and quantise(False, **{a: b}) == BAD, (a, b)
+    for a, b in (("codes", "scales"), ("codes", "zeros"), ("scales", "zeros")):
+        assert quantise(True, **{a: b}) == BAD, (a, b)
+    hip.sync()
+    for n, d in at.items():
+        assert (d.download() == 5).all(), n
+    assert product() == 0 and product(C="Y") == 0 and quantise(False) == 0 and quantise(True) == 0
+    hip.sync()
