@@ -329,6 +329,11 @@ def plan_q4(x_is_i8, M, N, K, group, workspace_bytes=0):
     return p
 
 
+def _in_a_row(v, count):
+    """Whether the DeviceMatrix v holds `count` fp32 values one behind the other."""
+    return v.dtype == np.float32 and v.rows * v.cols == count and (v.rows == 1 or v.pitch == v.cols)
+
+
 def gemm_q4(X, Q, Y, C=None, alpha=1.0, beta=1.0, x_scales=None, workspace=None, stream=None, plan=None):
     """Y = X . Q^T or fma(C, beta, alpha * X . Q^T) on DeviceMatrix operands; X fp16, or int8 with x_scales (M fp32 values);
     C of one row is added to every row of Y when Y has more.  plan: a Q4Plan to run on instead of the planner's."""
@@ -341,7 +346,7 @@ def gemm_q4(X, Q, Y, C=None, alpha=1.0, beta=1.0, x_scales=None, workspace=None,
     rest = (*Q.parts(), C.ptr if C is not None else None, Y.ptr, M, N, K, Q.group, X.pitch, ldc, Y.pitch, alpha, beta,
             1 if Y.dtype == np.float32 else 0, *ws, stream)
     if X.dtype == np.int8:
-        assert x_scales is not None and x_scales.dtype == np.float32 and x_scales.rows * x_scales.cols == M
+        assert x_scales is not None and _in_a_row(x_scales, M)
     else:
         assert X.dtype == np.float16 and x_scales is None
     if plan is not None:
@@ -355,10 +360,11 @@ def gemm_q4(X, Q, Y, C=None, alpha=1.0, beta=1.0, x_scales=None, workspace=None,
 
 def rmsnorm(x, weight, y, residual=None, sum_out=None, y_scales=None, eps=1e-5, stream=None):
     """y = h * weight / sqrt(mean(h^2) + eps) row by row, h = x + residual (kept in sum_out); y int8 with y_scales, or of x's type."""
-    assert x.dtype in (np.float16, np.float32) and weight.dtype == x.dtype and weight.cols == x.cols
-    assert y.dtype == (np.int8 if y_scales is not None else x.dtype)
-    for o in (y, residual, sum_out):
-        assert o is None or (o.rows, o.cols) == (x.rows, x.cols)
+    assert x.dtype in (np.float16, np.float32) and weight.dtype == x.dtype and (weight.rows, weight.cols) == (1, x.cols)
+    assert y.dtype == (np.int8 if y_scales is not None else x.dtype) and (y.rows, y.cols) == (x.rows, x.cols)
+    for o in (residual, sum_out):
+        assert o is None or ((o.rows, o.cols) == (x.rows, x.cols) and o.dtype == x.dtype)
+    assert y_scales is None or _in_a_row(y_scales, x.rows)
     fn = lib().decx_hip_rmsnorm_f16 if x.dtype == np.float16 else lib().decx_hip_rmsnorm_f32
     p = lambda m: (m.ptr, m.pitch) if m is not None else (None, 0)                          # noqa: E731
     check(fn(x.ptr, p(residual)[0], weight.ptr, p(sum_out)[0], y.ptr, p(y_scales)[0], x.rows, x.cols, x.pitch, p(residual)[1], p(sum_out)[1],

@@ -82,3 +82,36 @@ def test_operands_in_one_place_are_refused(i8):
         assert (d.download() == 5).all(), n
     assert product() == 0 and product(C="Y") == 0 and quantise(False) == 0 and quantise(True) == 0
     hip.sync()
+
+
+class Operand:
+    """What hip.gemm_q4 and hip.rmsnorm look at of a DeviceMatrix."""
+
+    def __init__(self, rows, cols, dtype, pitch=None):
+        self.rows, self.cols, self.dtype, self.pitch, self.ptr = rows, cols, np.dtype(dtype), pitch or cols, P(1 << 20)
+
+
+F16, F32, I8 = np.float16, np.float32, np.int8
+
+
+@pytest.mark.parametrize("change", [dict(y_scales=Operand(1, 3, F32)), dict(y_scales=Operand(1, 5, F32)), dict(y_scales=Operand(1, 4, F16)),
+                                    dict(y_scales=Operand(4, 1, F32, 2)), dict(weight=Operand(2, 8, F16)), dict(weight=Operand(1, 9, F16)),
+                                    dict(weight=Operand(1, 8, F32)), dict(residual=Operand(4, 8, F32)), dict(residual=Operand(3, 8, F16)),
+                                    dict(sum_out=Operand(4, 8, F32)), dict(sum_out=Operand(4, 9, F16)), dict(y=Operand(4, 8, F16)), dict(y=Operand(5, 8, I8))])
+def test_the_view_of_the_norm_checks_its_operands(change):
+    """(a y_scales of too few values would be written behind its end)"""
+    a = dict(x=Operand(4, 8, F16), weight=Operand(1, 8, F16), y=Operand(4, 8, I8), residual=Operand(4, 8, F16), sum_out=Operand(4, 8, F16), y_scales=Operand(1, 4, F32))
+    with pytest.raises(hip.HipError):                      # as it is it gets as far as the library, which has no device
+        hip.rmsnorm(**dict(a, y_scales=Operand(4, 1, F32), x=Operand(4, 8, F16, 7)))
+    with pytest.raises(AssertionError):
+        hip.rmsnorm(**dict(a, **change))
+
+
+@pytest.mark.parametrize("x_scales", [None, Operand(1, 3, F32), Operand(4, 1, F32, 3), Operand(1, 4, F16)])
+def test_the_view_of_the_product_checks_its_factors(x_scales):
+    q = Operand(6, 8, np.uint8)
+    q.group, q.parts = 64, lambda: (P(1 << 20), P(1 << 20), None)
+    with pytest.raises(AssertionError):
+        hip.gemm_q4(Operand(4, 8, I8), q, Operand(4, 6, F16), x_scales=x_scales)
+    with pytest.raises(hip.HipError):                      # (a pitch below the columns: refused by the library)
+        hip.gemm_q4(Operand(4, 8, I8), q, Operand(4, 6, F16, 5), x_scales=Operand(4, 1, F32))
