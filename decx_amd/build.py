@@ -68,9 +68,9 @@ def build_host(verbose=False):
 
 
 def build_api_test(verbose=False):
-    """The C++ programs the tests drive the public de:: API with (tests/cpp/de_api_test, linear4_test)."""
+    """The C++ programs the tests drive the public de:: API with (tests/cpp/de_api_test, linear4_test, linear4_edges_test)."""
     outs = []
-    for name in ("de_api_test", "linear4_test"):
+    for name in ("de_api_test", "linear4_test", "linear4_edges_test"):
         src = os.path.join(ROOT, "tests", "cpp", name + ".cpp")
         out = os.path.join(ROOT, "tests", "cpp", name)
         _run(["g++", "-O1", "-std=c++17", "-Wall", "-pthread", "-I" + os.path.join(ROOT, "include"), src, "-o", out,

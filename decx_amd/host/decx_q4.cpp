@@ -148,13 +148,15 @@ de::DH norm(de::GPU_Matrix& src, de::GPU_Matrix* residual, de::GPU_Vector& weigh
     if (r && (r->Width() != x->Width() || r->Height() != x->Height()))
         return failed(decx::DECX_FAIL_DimsNotMatching, "The source and the residual must be of the same size");
     if (!(eps >= 0.f) || !x->Width()) return failed(decx::DECX_FAIL_INVALID_PARAM, kInvalidParam);
-    // Outputs may lie in the storage of what has the same shape and type (then the same pitch, and re_construct keeps it), and
-    // of nothing else.
-    const auto shares = [](const decx::_GPU_Matrix* a, const decx::_GPU_Matrix* b) { return a && b && a != b && a->is_init() && b->is_init() && a->data() == b->data(); };
+    // Outputs may lie in the storage of an input of their own shape and type (then the same pitch, and re_construct keeps it),
+    // dst in the sum's whatever that was before (both are made that shape), and in nothing else.
+    const auto meets = [](const decx::_GPU_Matrix* a, const decx::_GPU_Matrix* b) {
+        return a && b && (a == b || (a->is_init() && b->is_init() && a->data() == b->data()));
+    };
     const auto same = [&](const decx::_GPU_Matrix* o) { return o->Type() == x->Type() && o->Width() == x->Width() && o->Height() == x->Height(); };
-    const bool clash_y = shares(y, x) || shares(y, r) || shares(y, h) || y == x || y == r || y == h;
-    const bool clash_h = shares(h, x) || shares(h, r);
-    if ((clash_y && (scales || !same(y))) || (h && clash_h && !same(h)) || (ys && ys->is_init() && ys->data() == w->data()))
+    const bool y_on_input = meets(y, x) || meets(y, r);
+    if ((ys && (y_on_input || meets(y, h))) || (y_on_input && !same(y)) || ((meets(h, x) || meets(h, r)) && !same(h)) ||
+        (ys && ys->is_init() && ys->data() == w->data()))
         return failed(decx::DECX_FAIL_INVALID_PARAM, kInvalidParam);
 
     std::lock_guard<std::mutex> guard(decx::module_mutex());

@@ -1,0 +1,104 @@
+// de::nn::cuda::Linear4, Quantize4 and RMSNorm at the edges of what their objects may be (needs a GPU).
+//   linear4_edges_test <name of a check>
+#include "DECX.h"
+
+#include <cmath>
+#include <cstring>
+#include <iostream>
+#include <string>
+#include <vector>
+
+static int g_failures = 0;
+#define CHECK(cond) do { if (!(cond)) { ++g_failures; std::cerr << "FAILED line " << __LINE__ << ": " #cond "\n"; } } while (0)
+
+static uint64_t g_seed = 777;
+static float uniform()                                    // [-1, 1), a multiple of 2^-7: exact in fp16
+{
+    g_seed = g_seed * 6364136223846793005ull + 1442695040888963407ull;
+    return (float)((int)(g_seed >> 56) - 128) / 128.f;
+}
+
+template <typename T> static T as(float v);
+template <> float as<float>(float v) { return v; }
+template <> de::Half as<de::Half>(float v) { return de::Float2Half(v); }
+static float of(float v) { return v; }
+static float of(de::Half v) { return de::Half2Float(v); }
+static float of(signed char v) { return v; }
+
+typedef std::vector<float> Values;                        // row after row
+
+template <typename T> static de::GPU_Matrix& upload(const Values& v, uint32_t w, uint32_t h, de::_DATA_TYPES_FLAGS_ type)
+{
+    de::Matrix& host = de::CreateMatrixRef(type, w, h);
+    for (uint32_t r = 0; r < h; ++r) for (uint32_t c = 0; c < w; ++c) *host.ptr<T>(r, c) = as<T>(v[(size_t)r * w + c]);
+    de::GPU_Matrix& dev = de::CreateGPUMatrixRef(type, w, h);
+    CHECK(de::Memcpy(host, dev, {0, 0}, {0, 0}, {(int)w, (int)h}, de::DECX_MEMCPY_H2D).error_type == 0);
+    host.release();
+    return dev;
+}
+template <typename T> static Values download(de::GPU_Matrix& dev)
+{
+    const uint32_t h = dev.Height(), w = dev.Width();
+    de::Matrix& host = de::CreateMatrixRef(dev.Type(), w, h);
+    CHECK(de::Memcpy(host, dev, {0, 0}, {0, 0}, {(int)w, (int)h}, de::DECX_MEMCPY_D2H).error_type == 0);
+    Values v((size_t)h * w);
+    for (uint32_t r = 0; r < h; ++r) for (uint32_t c = 0; c < w; ++c) v[(size_t)r * w + c] = of(*host.ptr<T>(r, c));
+    host.release();
+    return v;
+}
+static de::GPU_Vector& upload(const Values& v)
+{
+    de::Vector& host = de::CreateVectorRef(de::_FP16_, v.size());
+    for (size_t i = 0; i < v.size(); ++i) *host.ptr<de::Half>(i) = as<de::Half>(v[i]);
+    de::GPU_Vector& dev = de::CreateGPUVectorRef(de::_FP16_, v.size());
+    CHECK(de::Memcpy(host, dev, 0, 0, v.size(), de::DECX_MEMCPY_H2D).error_type == 0);
+    host.release();
+    return dev;
+}
+static Values random_values(size_t n)
+{
+    Values v(n);
+    for (float& e : v) e = uniform();
+    return v;
+}
+
+static const int kParam = decx::DECX_FAIL_INVALID_PARAM, kType = decx::DECX_FAIL_UNSUPPORTED_TYPE;
+
+// sum and dst one object, fresh or not: dst is written last
+static void dst_is_the_sum()
+{
+    const uint32_t w = 70, h = 5;
+    de::GPU_Matrix& x = upload<de::Half>(random_values(w * h), w, h, de::_FP16_);
+    de::GPU_Matrix& r = upload<de::Half>(random_values(w * h), w, h, de::_FP16_);
+    de::GPU_Vector& weight = upload(random_values(w));
+    de::GPU_Matrix& sum = de::CreateGPUMatrixRef();
+    de::GPU_Matrix& y = de::CreateGPUMatrixRef();
+    CHECK(de::nn::cuda::RMSNorm(x, r, weight, sum, y).error_type == 0);
+    const Values want = download<de::Half>(y);
+    de::GPU_Matrix& fresh = de::CreateGPUMatrixRef();
+    CHECK(de::nn::cuda::RMSNorm(x, r, weight, fresh, fresh).error_type == 0);
+    CHECK(fresh.Type() == de::_FP16_ && fresh.Width() == w && fresh.Height() == h && download<de::Half>(fresh) == want);
+    de::GPU_Matrix& other = upload<float>(random_values(300), 30, 10, de::_FP32_);          // of another shape and type, with room and without
+    CHECK(de::nn::cuda::RMSNorm(x, r, weight, other, other).error_type == 0 && download<de::Half>(other) == want);
+    de::GPU_Matrix& small = upload<float>(random_values(2), 2, 1, de::_FP32_);
+    de::GPU_Matrix& alias = de::CreateGPUMatrixRef();
+    alias.SoftCopy(small);
+    CHECK(de::nn::cuda::RMSNorm(x, r, weight, small, alias).error_type == 0 && download<de::Half>(alias) == want);
+    // codes cannot lie where the sum does
+    de::GPU_Matrix& none = de::CreateGPUMatrixRef();
+    de::GPU_Vector& scales = de::CreateGPUVectorRef();
+    CHECK(de::nn::cuda::RMSNorm(x, r, weight, none, none, scales).error_type == kParam && none.Width() == 0 && scales.Len() == 0);
+    // in place of the residual, and of the source, as before
+    CHECK(de::nn::cuda::RMSNorm(x, r, weight, r, r).error_type == 0 && download<de::Half>(r) == want);
+}
+
+
+int main(int argc, char** argv)
+{
+    const std::string name = argc > 1 ? argv[1] : "";
+    de::InitCuda();
+    if (name == "dst_is_the_sum") dst_is_the_sum();
+    else { std::cerr << "no such check\n"; return 2; }
+    std::cout << (g_failures ? "failed" : "ok") << std::endl;
+    return g_failures ? 1 : 0;
+}
