@@ -1224,7 +1224,7 @@ size_t decx_hip_q4_codes_bytes(uint32_t N, uint32_t K)
 
 size_t decx_hip_q4_scales_count(uint32_t N, uint32_t K, uint32_t group)
 {
-    if (group != 32 && group != 64 && group != 128) return 0;
+    if (!q4_shape_ok(N, K, group)) return 0;
     return decx_hip_q4_codes_bytes(N, K) / kQ4TileBytes * kQ4TileRows * (kQ4TileCols / group);
 }
 
@@ -1282,6 +1282,8 @@ static bool q4_product_ok(uint32_t M, uint32_t N, uint32_t K, uint32_t group)
     return q4_shape_ok(N, K, group) && N <= (1u << 25) && ((uint64_t)M / 64 + 1) * ((uint64_t)N / 128 + 1) <= (1u << 23);
 }
 
+int decx_hip_gemm_q4_fits(uint32_t M, uint32_t N, uint32_t K, uint32_t group) { return q4_product_ok(M, N, K, group) ? 1 : 0; }
+
 static int run_gemm_q4(bool i8, const void* X, const float* x_scales, const void* codes, const uint16_t* scales, const uint8_t* zeros,
                        const void* C, void* Y, uint32_t M, uint32_t N, uint32_t K, uint32_t group, uint32_t ldx, uint32_t ldc, uint32_t ldy,
                        float alpha, float beta, int y_is_f32, void* workspace, size_t workspace_bytes, void* stream, const GemmQ4Plan* forced = nullptr)
@@ -1332,7 +1334,7 @@ int decx_hip_gemm_q4_i8(const int8_t* X, const float* x_scales, const void* code
 
 size_t decx_hip_gemm_q4_workspace(int x_is_i8, uint32_t M, uint32_t N, uint32_t K, uint32_t group)
 {
-    if (M == 0 || N == 0 || K == 0 || !q4_shape_ok(N, K, group)) return 0;
+    if (M == 0 || N == 0 || K == 0 || !q4_product_ok(M, N, K, group)) return 0;
     return gemm_q4_workspace(x_is_i8 != 0, group, M, N, K);
 }
 

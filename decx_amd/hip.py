@@ -80,6 +80,7 @@ SYMBOLS = {
     "decx_hip_q4_quantize_f16": (_int, [_vp] * 4 + [_u32] * 4 + [_vp]),
     "decx_hip_q4_dequantize_f32": (_int, [_vp] * 4 + [_u32] * 4 + [_vp]),
     "decx_hip_q4_dequantize_f16": (_int, [_vp] * 4 + [_u32] * 4 + [_vp]),
+    "decx_hip_gemm_q4_fits": (_int, [_u32] * 4),
     "decx_hip_gemm_q4_workspace": (_sz, [_int] + [_u32] * 4),
     "decx_hip_gemm_q4_f16": (_int, [_vp] * 6 + [_u32] * 7 + [_f, _f, _int, _vp, _sz, _vp]),
     "decx_hip_gemm_q4_i8": (_int, [_vp] * 7 + [_u32] * 7 + [_f, _f, _int, _vp, _sz, _vp]),

@@ -106,6 +106,7 @@ de::DH linear(de::GPU_Matrix& src, de::GPU_Vector* src_scales, de::GPU_Matrix4& 
     // dst must not write over what is still read: its storage is the source's, or that of a row that all rows add
     if (y->is_init() && (y->data() == x->data() || (c && y->data() == c->data() && (c->Height() != x->Height() || y->Pitch() != c->Pitch() || y->Type() != c->Type()))))
         return failed(decx::DECX_FAIL_INVALID_PARAM, kInvalidParam);
+    if (!decx_hip_gemm_q4_fits(x->Height(), w->Height(), w->Width(), w->Group())) return failed(decx::DECX_FAIL_INVALID_PARAM, kInvalidParam);
     const bool f32 = c ? c->Type() == de::_FP32_ : accu == de::Fp16_Accurate_L1;
 
     std::lock_guard<std::mutex> guard(decx::module_mutex());
@@ -147,7 +148,7 @@ de::DH norm(de::GPU_Matrix& src, de::GPU_Matrix* residual, de::GPU_Vector& weigh
     if (w->Len() != x->Width()) return failed(decx::DECX_FAIL_DimsNotMatching, "There must be one weight for every column of the source");
     if (r && (r->Width() != x->Width() || r->Height() != x->Height()))
         return failed(decx::DECX_FAIL_DimsNotMatching, "The source and the residual must be of the same size");
-    if (!(eps >= 0.f) || !x->Width()) return failed(decx::DECX_FAIL_INVALID_PARAM, kInvalidParam);
+    if (!(eps >= 0.f) || !x->Width() || x->Width() > 0xffff0000u || x->Height() > 0x7fffffffu) return failed(decx::DECX_FAIL_INVALID_PARAM, kInvalidParam);
     // Outputs may lie in the storage of an input of their own shape and type (then the same pitch, and re_construct keeps it),
     // dst in the sum's whatever that was before (both are made that shape), and in nothing else.
     const auto meets = [](const decx::_GPU_Matrix* a, const decx::_GPU_Matrix* b) {

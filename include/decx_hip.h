@@ -312,7 +312,8 @@ DECX_HIP_API int decx_hip_conv2d_f32_depth(const float* image, const float* kmat
  *           scales of one row of a tile (256 / group bytes);
  *   zeros   as many bytes in the same order, aligned to 128 / group, or NULL: 8 everywhere. */
 DECX_HIP_API size_t decx_hip_q4_codes_bytes(uint32_t N, uint32_t K);
-DECX_HIP_API size_t decx_hip_q4_scales_count(uint32_t N, uint32_t K, uint32_t group);   /* 0 for any other group */
+DECX_HIP_API size_t decx_hip_q4_scales_count(uint32_t N, uint32_t K, uint32_t group);   /* 0 for any other group, and for a
+                                            matrix that no call takes: more than 2^26 - 4 tiles, N or K above 2^32 - 256 */
 
 /* Makes a 4-bit matrix of W (N x K, row pitch ldw).  Per group, over its columns that exist:
  *   zeros == NULL:  scale = max|w| / 7,  code = clamp(rint(w / scale), -8, 7) + 8
@@ -346,6 +347,8 @@ DECX_HIP_API int decx_hip_q4_dequantize_f16(const void* codes, const uint16_t* s
  * decx_hip_gemm_q4_workspace says how many bytes are of use (0: none).  It must be 16-byte aligned and is free again when
  * the call's work on `stream` is done; calls that may overlap -- other streams, graphs replayed side by side -- each need
  * their own.  Results do not depend on timing, but may differ in rounding with and without it. */
+/* 1 if a product of these sizes is taken, 0 if it is refused for them (to be asked before memory is set aside for it). */
+DECX_HIP_API int decx_hip_gemm_q4_fits(uint32_t M, uint32_t N, uint32_t K, uint32_t group);
 DECX_HIP_API size_t decx_hip_gemm_q4_workspace(int x_is_i8, uint32_t M, uint32_t N, uint32_t K, uint32_t group);
 DECX_HIP_API int decx_hip_gemm_q4_f16(const uint16_t* X, const void* codes, const uint16_t* scales, const uint8_t* zeros,
                                       const void* C, void* Y, uint32_t M, uint32_t N, uint32_t K, uint32_t group,

@@ -93,11 +93,35 @@ static void dst_is_the_sum()
 }
 
 
+// sizes that the entry points below refuse: found out before the outputs are made anew
+static void sizes_that_are_refused()
+{
+    de::GPU_Matrix& tall = de::CreateGPUMatrixRef(de::_FP16_, 1, 1u << 30);
+    de::GPU_Matrix4& q = de::CreateGPUMatrix4Ref();
+    CHECK(de::nn::cuda::Quantize4(tall, q).error_type == kParam && q.Width() == 0 && q.Height() == 0);      // 2^26 tiles
+    tall.release();
+    de::GPU_Matrix& outputs = de::CreateGPUMatrixRef(de::_FP16_, 1, (1u << 25) + 1);
+    CHECK(de::nn::cuda::Quantize4(outputs, q).error_type == 0 && q.Height() == (1u << 25) + 1);
+    de::GPU_Matrix& x = upload<de::Half>(random_values(2), 1, 2, de::_FP16_);
+    de::GPU_Matrix& y = de::CreateGPUMatrixRef();
+    CHECK(de::nn::cuda::Linear4(x, q, y).error_type == kParam && y.Width() == 0 && y.Height() == 0 && y.Type() == de::_VOID_);
+    q.release();
+    outputs.release();
+    de::GPU_Matrix& rows = de::CreateGPUMatrixRef(de::_FP16_, 1, 1u << 31);
+    de::GPU_Vector& weight = upload(random_values(1));
+    de::GPU_Vector& scales = de::CreateGPUVectorRef();
+    CHECK(de::nn::cuda::RMSNorm(rows, weight, y).error_type == kParam && y.Width() == 0);
+    CHECK(de::nn::cuda::RMSNorm(rows, weight, y, scales).error_type == kParam && y.Width() == 0 && scales.Len() == 0);
+    rows.release();
+}
+
+
 int main(int argc, char** argv)
 {
     const std::string name = argc > 1 ? argv[1] : "";
     de::InitCuda();
     if (name == "dst_is_the_sum") dst_is_the_sum();
+    else if (name == "sizes_that_are_refused") sizes_that_are_refused();
     else { std::cerr << "no such check\n"; return 2; }
     std::cout << (g_failures ? "failed" : "ok") << std::endl;
     return g_failures ? 1 : 0;

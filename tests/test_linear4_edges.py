@@ -17,3 +17,8 @@ def run(check):
 @pytest.mark.gpu
 def test_the_norm_of_a_sum_may_lie_where_the_sum_does():
     run("dst_is_the_sum")
+
+
+@pytest.mark.gpu
+def test_sizes_that_are_refused_leave_the_outputs_as_they_were():
+    run("sizes_that_are_refused")

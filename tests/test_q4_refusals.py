@@ -115,3 +115,16 @@ def test_the_view_of_the_product_checks_its_factors(x_scales):
         hip.gemm_q4(Operand(4, 8, I8), q, Operand(4, 6, F16), x_scales=x_scales)
     with pytest.raises(hip.HipError):                      # (a pitch below the columns: refused by the library)
         hip.gemm_q4(Operand(4, 8, I8), q, Operand(4, 6, F16, 5), x_scales=Operand(4, 1, F32))
+
+
+def test_sizes_are_known_beforehand():
+    """What decx_hip_gemm_q4_fits, the workspace's and the scales' sizes say of products and matrices that are refused."""
+    L = hip.lib()
+    for M, N, K, group in ((1, (1 << 25) + 1, 128, 64), (1 << 31, 1 << 20, 128, 64), (0xffffffff, 0xffffff00, 128, 64), (0xffffffff, 1, 128, 64), (1 << 29, 128, 4096, 64),
+                           (4, 20, 0xffffff80, 64), (4, 20, 130, 48), (4, 960, 1118481 * 128 + 1, 64)):
+        assert L.decx_hip_gemm_q4_fits(M, N, K, group) == 0 and L.decx_hip_gemm_q4_workspace(0, M, N, K, group) == 0, (M, N, K, group)
+    for M, N, K, group in ((1, 1 << 25, 128, 64), (0, 5, 0, 32), ((1 << 29) - 65, 100, 300, 128), (65, 300, 4100, 128)):
+        assert L.decx_hip_gemm_q4_fits(M, N, K, group) == 1
+    assert L.decx_hip_gemm_q4_workspace(0, 65, 300, 4100, 128) > 0
+    assert L.decx_hip_q4_scales_count(960, 1118481 * 128, 32) == ((1 << 26) - 4) * 64 and L.decx_hip_q4_scales_count(960, 1118481 * 128 + 1, 32) == 0
+    assert L.decx_hip_q4_scales_count(0xffffff01, 128, 64) == 0
