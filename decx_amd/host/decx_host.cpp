@@ -156,7 +156,8 @@ de::_DATA_FORMATS_ decx::_Matrix::Format() const { return _format; }
 de::Matrix& decx::_Matrix::SoftCopy(de::Matrix& src)
 {
     const _Matrix& s = dynamic_cast<_Matrix&>(src);
-    assign(s._type, s._layout.width, s._layout.height);
+    _type = s._type;
+    _layout = s._layout;               // (that of the storage, whatever type it was given since)
     _format = s._format;
     _block = s._block;                 // shared, reference counted
     _data = s._data;
@@ -165,7 +166,8 @@ de::Matrix& decx::_Matrix::SoftCopy(de::Matrix& src)
 
 void decx::_Matrix::re_construct(de::_DATA_TYPES_FLAGS_ type, uint32_t width, uint32_t height)
 {
-    if (_type == type && _layout.width == width && _layout.height == height && _data) return;
+    // (after Reinterpret the storage may be that of smaller elements)
+    if (_type == type && _layout.width == width && _layout.height == height && _data && _layout._single_element_size == (int32_t)element_size(type)) return;
     const size_t before = _block ? _block->bytes : 0;
     assign(type, width, height);
     if (total_bytes() > before || !_data) allocate();
@@ -284,7 +286,8 @@ de::_DATA_FORMATS_ decx::_GPU_Matrix::Format() const { return _format; }
 de::GPU_Matrix& decx::_GPU_Matrix::SoftCopy(de::GPU_Matrix& src)
 {
     const _GPU_Matrix& s = dynamic_cast<_GPU_Matrix&>(src);
-    assign(s._type, s._layout.width, s._layout.height);
+    _type = s._type;
+    _layout = s._layout;               // (that of the storage, whatever type it was given since)
     _format = s._format;
     _block = s._block;
     return *this;
@@ -292,10 +295,17 @@ de::GPU_Matrix& decx::_GPU_Matrix::SoftCopy(de::GPU_Matrix& src)
 
 bool decx::_GPU_Matrix::re_construct(de::_DATA_TYPES_FLAGS_ type, uint32_t width, uint32_t height)
 {
-    if (_type == type && _layout.width == width && _layout.height == height && is_init()) return true;
+    // (after Reinterpret the storage may be that of smaller elements)
+    if (_type == type && _layout.width == width && _layout.height == height && is_init() && _layout._single_element_size == (int32_t)element_size(type)) return true;
     const size_t before = _block ? _block->bytes : 0;
+    const de::MatrixLayout old_layout = _layout;
+    const de::_DATA_TYPES_FLAGS_ old_type = _type;
     assign(type, width, height);
-    if (total_bytes() > before || !is_init()) return allocate();
+    if ((total_bytes() > before || !is_init()) && !allocate()) {       // what it was it stays: its storage has room for that alone
+        _layout = old_layout;
+        _type = old_type;
+        return false;
+    }
     return true;
 }
 

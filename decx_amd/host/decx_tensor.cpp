@@ -130,7 +130,8 @@ de::DH decx::_GPU_Tensor::Extract_SoftCopy(const uint32_t, de::GPU_Tensor&) cons
 }
 bool decx::_GPU_Tensor::re_construct(de::_DATA_TYPES_FLAGS_ type, uint32_t width, uint32_t height, uint32_t depth)
 {
-    if (_type == type && _layout.width == width && _layout.height == height && _layout.depth == depth && _data) return true;
+    if (_type == type && _layout.width == width && _layout.height == height && _layout.depth == depth && _data &&
+        _layout._single_element_size == (int32_t)element_size(type)) return true;
     // a view into someone else's storage (Extract_SoftCopy) is never reshaped in place
     const bool own = _block && _data == _block->ptr;
     const size_t before = own ? _block->bytes : 0;

@@ -63,7 +63,7 @@ void decx::_Vector::Reinterpret(const de::_DATA_TYPES_FLAGS_ t) { _type = t; }
 de::Vector& decx::_Vector::SoftCopy(de::Vector& src)
 {
     const _Vector& s = dynamic_cast<_Vector&>(src);
-    assign(s._type, s._length);
+    _type = s._type; _element_size = s._element_size; _length = s._length; _capacity = s._capacity;
     _block = s._block;
     _data = s._data;
     return *this;
@@ -71,7 +71,7 @@ de::Vector& decx::_Vector::SoftCopy(de::Vector& src)
 
 bool decx::_Vector::re_construct(de::_DATA_TYPES_FLAGS_ type, size_t length)
 {
-    if (_type == type && _length == length && _data) return true;
+    if (_type == type && _length == length && _data && _element_size == element_size(type)) return true;     // (not so after Reinterpret)
     const size_t before = _block ? _block->bytes : 0;
     assign(type, length);
     if (_capacity * _element_size > before || !_data) return allocate();
@@ -173,17 +173,26 @@ void decx::_GPU_Vector::Reinterpret(const de::_DATA_TYPES_FLAGS_ t) { _type = t;
 de::GPU_Vector& decx::_GPU_Vector::SoftCopy(de::GPU_Vector& src)
 {
     const _GPU_Vector& s = dynamic_cast<_GPU_Vector&>(src);
-    assign(s._type, s._length);
+    _type = s._type; _element_size = s._element_size; _length = s._length; _capacity = s._capacity;
     _block = s._block;
     return *this;
 }
 
 bool decx::_GPU_Vector::re_construct(de::_DATA_TYPES_FLAGS_ type, size_t length)
 {
-    if (_type == type && _length == length && is_init()) return true;
+    if (_type == type && _length == length && is_init() && _element_size == element_size(type)) return true;  // (not so after Reinterpret)
     const size_t before = _block ? _block->bytes : 0;
+    const size_t old_length = _length;
+    const uint32_t old_size = _element_size;
+    const de::_DATA_TYPES_FLAGS_ old_type = _type;
     assign(type, length);
-    if (_capacity * _element_size > before || !is_init()) return allocate();
+    if ((_capacity * _element_size > before || !is_init()) && !allocate()) {        // what it was it stays
+        _type = old_type;
+        _element_size = old_size;
+        _length = old_length;
+        _capacity = aligned_length(_length, _element_size);
+        return false;
+    }
     return true;
 }
 

@@ -115,6 +115,31 @@ static void sizes_that_are_refused()
     rows.release();
 }
 
+// outputs that were given another type before: storage of smaller elements is not taken for one of larger
+static void outputs_of_another_type()
+{
+    const uint32_t w = 64, h = 200;
+    de::GPU_Matrix& x = upload<de::Half>(random_values(w * h), w, h, de::_FP16_);
+    de::GPU_Vector& weight = upload(random_values(w));
+    de::GPU_Matrix& y = de::CreateGPUMatrixRef();
+    de::GPU_Matrix& codes = de::CreateGPUMatrixRef();
+    de::GPU_Vector& scales = de::CreateGPUVectorRef();
+    CHECK(de::nn::cuda::RMSNorm(x, weight, y).error_type == 0 && de::nn::cuda::RMSNorm(x, weight, codes, scales).error_type == 0);
+    const Values want = download<de::Half>(y), want_codes = download<signed char>(codes);
+    de::GPU_Matrix& narrow = de::CreateGPUMatrixRef(de::_UINT8_, w, h);
+    narrow.Reinterpret(de::_FP16_);
+    CHECK(de::nn::cuda::RMSNorm(x, weight, narrow).error_type == 0 && download<de::Half>(narrow) == want);
+    de::GPU_Matrix& wide = de::CreateGPUMatrixRef(de::_FP32_, w, h);
+    wide.Reinterpret(de::_UINT8_);
+    de::GPU_Vector& halves = de::CreateGPUVectorRef(de::_FP16_, h);
+    halves.Reinterpret(de::_FP32_);
+    CHECK(de::nn::cuda::RMSNorm(x, weight, wide, halves).error_type == 0 && download<signed char>(wide) == want_codes);
+    de::Vector& a = de::CreateVectorRef(de::_FP32_, h);
+    de::Vector& b = de::CreateVectorRef(de::_FP32_, h);
+    CHECK(de::Memcpy(a, scales, 0, 0, h, de::DECX_MEMCPY_D2H).error_type == 0 && de::Memcpy(b, halves, 0, 0, h, de::DECX_MEMCPY_D2H).error_type == 0);
+    for (uint32_t i = 0; i < h; ++i) CHECK(*a.ptr<float>(i) == *b.ptr<float>(i));
+}
+
 
 int main(int argc, char** argv)
 {
@@ -122,6 +147,7 @@ int main(int argc, char** argv)
     de::InitCuda();
     if (name == "dst_is_the_sum") dst_is_the_sum();
     else if (name == "sizes_that_are_refused") sizes_that_are_refused();
+    else if (name == "outputs_of_another_type") outputs_of_another_type();
     else { std::cerr << "no such check\n"; return 2; }
     std::cout << (g_failures ? "failed" : "ok") << std::endl;
     return g_failures ? 1 : 0;
