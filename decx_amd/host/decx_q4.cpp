@@ -77,6 +77,10 @@ decx::DeviceBlock* workspace(size_t need)
     return kept.get();
 }
 
+// An input that was given another type (Reinterpret) keeps its pitch and storage: only elements of the same size are still there.
+bool whole(const decx::_GPU_Matrix* m) { return !m || decx::element_size(m->Type()) == (uint32_t)m->get_layout()._single_element_size; }
+bool whole(const decx::_GPU_Vector* v) { return !v || decx::element_size(v->Type()) == v->element_bytes(); }
+
 float scalar_of(const de::Number& n) { return n.Type() == de::_FP16_ ? de::Half2Float(n.get_data_ref<de::Half>()) : n.get_data_ref<float>(); }
 
 de::DH linear(de::GPU_Matrix& src, de::GPU_Vector* src_scales, de::GPU_Matrix4& weights, de::GPU_Matrix* C, de::GPU_Matrix& dst,
@@ -91,7 +95,8 @@ de::DH linear(de::GPU_Matrix& src, de::GPU_Vector* src_scales, de::GPU_Matrix4& 
     if (!decx::gpu_ready()) return failed(decx::DECX_FAIL_CUDA_not_init, kCudaNotInit);
     if (!x || !w || !y || !x->is_init() || !w->is_init() || (src_scales && (!xs || !xs->is_init())) || (C && (!c || !c->is_init())))
         return failed(decx::DECX_FAIL_CLASS_NOT_INIT, kClassNotInit);
-    if (x->Type() != (xs ? de::_UINT8_ : de::_FP16_) || (xs && xs->Type() != de::_FP32_) || (c && c->Type() != de::_FP16_ && c->Type() != de::_FP32_))
+    if (x->Type() != (xs ? de::_UINT8_ : de::_FP16_) || (xs && xs->Type() != de::_FP32_) || (c && c->Type() != de::_FP16_ && c->Type() != de::_FP32_) || !whole(x) || !whole(xs) ||
+        !whole(c))
         return failed(decx::DECX_FAIL_UNSUPPORTED_TYPE, kUnsupportedType);
     if (accu > de::Fp16_Accurate_L3) return failed(decx::DECX_FAIL_INVALID_PARAM, kInvalidParam);
     if (x->Width() != w->Width())
@@ -143,7 +148,7 @@ de::DH norm(de::GPU_Matrix& src, de::GPU_Matrix* residual, de::GPU_Vector& weigh
     if (!decx::gpu_ready()) return failed(decx::DECX_FAIL_CUDA_not_init, kCudaNotInit);
     if (!x || !w || !y || !x->is_init() || !w->is_init() || (residual && (!r || !r->is_init())) || (sum && !h) || (scales && !ys))
         return failed(decx::DECX_FAIL_CLASS_NOT_INIT, kClassNotInit);
-    if (x->Type() != de::_FP16_ && x->Type() != de::_FP32_) return failed(decx::DECX_FAIL_UNSUPPORTED_TYPE, kUnsupportedType);
+    if ((x->Type() != de::_FP16_ && x->Type() != de::_FP32_) || !whole(x) || !whole(r) || !whole(w)) return failed(decx::DECX_FAIL_UNSUPPORTED_TYPE, kUnsupportedType);
     if (w->Type() != x->Type() || (r && r->Type() != x->Type())) return failed(decx::DECX_FAIL_TYPE_MOT_MATCH, kTypeNotMatch);
     if (w->Len() != x->Width()) return failed(decx::DECX_FAIL_DimsNotMatching, "There must be one weight for every column of the source");
     if (r && (r->Width() != x->Width() || r->Height() != x->Height()))
@@ -192,7 +197,7 @@ _DECX_API_ de::DH de::nn::cuda::Quantize4(de::GPU_Matrix& src, de::GPU_Matrix4& 
     decx::_GPU_Matrix4* d = dynamic_cast<decx::_GPU_Matrix4*>(&dst);
     if (!decx::gpu_ready()) return failed(decx::DECX_FAIL_CUDA_not_init, kCudaNotInit);
     if (!s || !d || !s->is_init()) return failed(decx::DECX_FAIL_CLASS_NOT_INIT, kClassNotInit);
-    if (s->Type() != de::_FP16_ && s->Type() != de::_FP32_) return failed(decx::DECX_FAIL_UNSUPPORTED_TYPE, kUnsupportedType);
+    if ((s->Type() != de::_FP16_ && s->Type() != de::_FP32_) || !whole(s)) return failed(decx::DECX_FAIL_UNSUPPORTED_TYPE, kUnsupportedType);
     if (!s->Width() || !s->Height() || !decx_hip_q4_scales_count(s->Height(), s->Width(), group)) return failed(decx::DECX_FAIL_INVALID_PARAM, kInvalidParam);
     std::lock_guard<std::mutex> guard(decx::module_mutex());
     if (!d->re_construct(s->Width(), s->Height(), group, zeros)) return failed(decx::DECX_FAIL_CUDA_ALLOCATION, kDevAllocFail);

@@ -140,6 +140,53 @@ static void outputs_of_another_type()
     for (uint32_t i = 0; i < h; ++i) CHECK(*a.ptr<float>(i) == *b.ptr<float>(i));
 }
 
+// inputs that were given another type: of another size refused, of the same one taken for what they are
+static void inputs_of_another_type()
+{
+    const uint32_t w = 64, h = 4, n = 32;
+    const Values values = random_values(w * h);
+    de::GPU_Matrix& x = upload<de::Half>(values, w, h, de::_FP16_);
+    de::GPU_Matrix& weights = upload<float>(random_values(w * n), w, n, de::_FP32_);
+    de::GPU_Vector& weight = upload(random_values(w));
+    de::GPU_Matrix4& q = de::CreateGPUMatrix4Ref();
+    de::GPU_Matrix& y = de::CreateGPUMatrixRef();
+    de::GPU_Vector& scales = de::CreateGPUVectorRef(de::_FP32_, h);
+    de::GPU_Matrix& codes = de::CreateGPUMatrixRef(de::_UINT8_, w, h);
+    CHECK(de::nn::cuda::Quantize4(weights, q).error_type == 0);
+    de::GPU_Matrix& b16 = upload<de::Half>(values, w, h, de::_FP16_);
+    b16.Reinterpret(de::_FP32_);
+    de::GPU_Matrix& b8 = de::CreateGPUMatrixRef(de::_UINT8_, w, h);
+    b8.Reinterpret(de::_FP16_);
+    de::GPU_Matrix& c16 = de::CreateGPUMatrixRef(de::_FP16_, n, h);
+    c16.Reinterpret(de::_FP32_);
+    de::GPU_Vector& v16 = de::CreateGPUVectorRef(de::_FP16_, h);
+    v16.Reinterpret(de::_FP32_);
+    de::GPU_Vector& w8 = de::CreateGPUVectorRef(de::_UINT8_, w);
+    w8.Reinterpret(de::_FP16_);
+    CHECK(de::nn::cuda::Linear4(b8, q, y).error_type == kType);
+    de::GPU_Matrix& alias = de::CreateGPUMatrixRef();
+    alias.SoftCopy(b8);
+    CHECK(de::nn::cuda::Linear4(alias, q, y).error_type == kType && de::nn::cuda::RMSNorm(alias, weight, y).error_type == kType);
+    CHECK(de::nn::cuda::Linear4(x, q, c16, y, de::Number(1.f), de::Number(1.f)).error_type == kType);
+    CHECK(de::nn::cuda::Linear4(codes, v16, q, y).error_type == kType);
+    CHECK(de::nn::cuda::RMSNorm(b8, weight, y).error_type == kType && de::nn::cuda::RMSNorm(x, w8, y).error_type == kType);
+    CHECK(de::nn::cuda::RMSNorm(x, b8, weight, y, codes).error_type == kType && codes.Type() == de::_UINT8_);
+    de::GPU_Matrix4& none = de::CreateGPUMatrix4Ref();
+    CHECK(de::nn::cuda::Quantize4(b16, none).error_type == kType && none.Width() == 0 && y.Width() == 0);
+    CHECK(de::nn::cuda::Linear4(codes, scales, q, y).error_type == 0);
+    de::GPU_Matrix& f32 = upload<float>(values, w, h, de::_FP32_);
+    de::GPU_Matrix4& q1 = de::CreateGPUMatrix4Ref();
+    de::GPU_Matrix4& q2 = de::CreateGPUMatrix4Ref();
+    CHECK(de::nn::cuda::Quantize4(f32, q1).error_type == 0);
+    f32.Reinterpret(de::_INT32_);
+    f32.Reinterpret(de::_FP32_);
+    CHECK(de::nn::cuda::Quantize4(f32, q2).error_type == 0);
+    de::GPU_Matrix& v1 = de::CreateGPUMatrixRef();
+    de::GPU_Matrix& v2 = de::CreateGPUMatrixRef();
+    CHECK(de::nn::cuda::Dequantize4(q1, v1).error_type == 0 && de::nn::cuda::Dequantize4(q2, v2).error_type == 0);
+    CHECK(download<de::Half>(v1) == download<de::Half>(v2));
+}
+
 
 int main(int argc, char** argv)
 {
@@ -148,6 +195,7 @@ int main(int argc, char** argv)
     if (name == "dst_is_the_sum") dst_is_the_sum();
     else if (name == "sizes_that_are_refused") sizes_that_are_refused();
     else if (name == "outputs_of_another_type") outputs_of_another_type();
+    else if (name == "inputs_of_another_type") inputs_of_another_type();
     else { std::cerr << "no such check\n"; return 2; }
     std::cout << (g_failures ? "failed" : "ok") << std::endl;
     return g_failures ? 1 : 0;

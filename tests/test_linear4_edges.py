@@ -38,3 +38,8 @@ def test_storage_of_objects_that_are_made_anew(tmp_path):
 @pytest.mark.gpu
 def test_outputs_that_were_given_another_type():
     run("outputs_of_another_type")
+
+
+@pytest.mark.gpu
+def test_inputs_that_were_given_another_type():
+    run("inputs_of_another_type")
