@@ -3,7 +3,8 @@
 //   h = x + residual (rounded to the rows' type, kept if asked for),  rho = 1 / sqrt(mean(h^2) + eps),  y = h * weight * rho
 //   8 bits: top = max |h * weight| over the row,  code = rint(127 * h * weight / top),  scale = top * rho / 127
 //
-// rho cancels out of the codes, so they depend on h * weight alone: exact in fp32 for fp16 rows, in 64 bits for fp32 rows.
+// rho cancels out of the codes, so they depend on h * weight alone: exact in fp32 for fp16 rows, in 64 bits for fp32 rows.  A
+// quotient next to a half is decided by exact products, so no code depends on how one was rounded.
 // Sums of squares are kept in fp32 for fp16 rows (a row cannot overflow it) and in 64 bits for fp32 rows (it could).
 // Bound: HBM.  A workgroup owns a row and holds h in registers between the two passes over it; rows too long for that are
 // read a second time (from the kept sum where there is one).  4096 x 8192 fp16 with residual, sum and 8 bits out: 46.0 us, 5.1 TB/s
@@ -59,13 +60,18 @@ template <typename T> __device__ __forceinline__ void store_chunk(T* row, uint32
 __device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint64_t max_of(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
-// rint(127 t / top) by comparison with the half top (m + 1/2) next to the quotient, m = floor(v), v the quotient in fp32: both
-// products are exact in 64 bits for fp16 rows.
-__device__ __forceinline__ float rint_exactly(double t, double top, float v)
+// rint(127 t / top) by comparison with the half top (m + 1/2) next to the quotient, m = floor(v), v the quotient in fp32.  t and
+// top are products of two elements: of fp16 ones 22 bits, and both sides are exact in 64 bits; of fp32 ones 48 bits, the sides take
+// up to 56, and what each lost is compared behind them (the fma gives it exactly, and so is the difference of two such ends; the
+// sides' own difference is exact next to a half, elsewhere larger than what they lost).
+template <bool ENDS> __device__ __forceinline__ float rint_exactly(double t, double top, float v)
 {
+#pragma clang fp contract(off)                             // (the difference is that of the rounded sides)
     const float m = __builtin_floorf(v), even = 2.f * __builtin_rintf(0.5f * m + 0.25f);      // of m and m + 1 the even one
     const double left = 127.0 * t, half = top * (double)(m + 0.5f);
-    return left > half ? m + 1.f : (left < half ? m : even);
+    double above = left - half;
+    if constexpr (ENDS) above += __builtin_fma(127.0, t, -left) - __builtin_fma(top, (double)(m + 0.5f), -half);
+    return above > 0 ? m + 1.f : (above < 0 ? m : even);
 }
 
 }  // namespace
@@ -161,7 +167,7 @@ rmsnorm_kernel(const RmsNormArgs g)
             }
             if (near < 4e-5f) {
 #pragma unroll
-                for (int e = 0; e < n; ++e) c[e] = rint_exactly((double)((wide)h[e] * (wide)wv[e]), (double)most, v[e]);
+                for (int e = 0; e < n; ++e) c[e] = rint_exactly<sizeof(T) == 4>((double)((wide)h[e] * (wide)wv[e]), (double)most, v[e]);
             }
 #pragma unroll
             for (int e = 0; e < n; ++e) word[e / 4] |= ((uint32_t)(int)c[e] & 0xffu) << (8 * (e % 4));

@@ -1,0 +1,48 @@
+"""The root-mean-square norm where rounding decides: against whole numbers and fractions."""
+from fractions import Fraction
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def hip():
+    from decx_amd import hip as h
+    h.init()
+    return h
+
+
+def rint(q):
+    """A fraction to the nearest whole number, halves to the even one."""
+    low = q.numerator // q.denominator
+    rest = q - low
+    return low + 1 if rest > Fraction(1, 2) or (rest == Fraction(1, 2) and low % 2) else low
+
+
+# (top's factors, t's factors): fp32 values whose 127 t / top misses a half by less than the last of 53 bits of either side
+NEXT_TO_A_HALF = [(10826011, 12636473, 8806181, 13883497), (15460537, 15476367, 11702938, 16018360), (12190991, 11474615, 9030521, 12258199),
+                  (10152001, 16244053, 11760712, 12862774), (11945017, 13029605, 9362068, 15773554), (11300127, 12203409, 6023476, 12889012),
+                  (10959887, 10180709, 3832792, 13180533), (16618719, 10210709, 4910714, 8570687)]
+
+
+@pytest.mark.parametrize("cols", [2, 4, 300, 5001, 40001])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -60, 2.0 ** 70])
+def test_codes_of_fp32_rows_next_to_a_half(hip, cols, scale):
+    """Products of 48 bits: the sides of the comparison do not fit 64-bit floating point."""
+    for a, b, c, d in NEXT_TO_A_HALF:
+        left = rint(Fraction(127 * c * d, a * b))
+        exactly = Fraction(127 * c * d, a * b) - Fraction(127 * c * d * 2 // (a * b), 2)
+        assert min(exactly, Fraction(1, 2) - exactly) < Fraction(1, 1 << 44)
+        x, w = np.zeros((2, cols), np.float32), np.ones((1, cols), np.float32)
+        at, top = cols // 3, cols - 1
+        x[:, top], w[0, top] = a * scale, b
+        x[0, at], x[1, at], w[0, at] = c * scale, -c * scale, d
+        dx, dw = hip.DeviceMatrix(2, cols, np.float32, data=x), hip.DeviceMatrix(1, cols, np.float32, data=w)
+        dy, ds = hip.DeviceMatrix(2, cols, np.int8, pad_value=77), hip.DeviceMatrix(1, 2, np.float32)
+        hip.rmsnorm(dx, dw, dy, y_scales=ds)
+        hip.sync()
+        want = np.zeros((2, cols), np.int8)
+        want[:, top], want[0, at], want[1, at] = 127, left, -left
+        assert np.array_equal(dy.download(), want), (a, b, c, d)
