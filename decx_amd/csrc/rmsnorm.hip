@@ -5,7 +5,8 @@
 //
 // rho cancels out of the codes, so they depend on h * weight alone: exact in fp32 for fp16 rows, in 64 bits for fp32 rows.  A
 // quotient next to a half is decided by exact products, so no code depends on how one was rounded.
-// Sums of squares are kept in fp32 for fp16 rows (a row cannot overflow it) and in 64 bits for fp32 rows (it could).
+// Sums of squares are kept in fp32 for fp16 rows (a row cannot overflow it; of rows that are read twice only those of 8 elements and
+// what a workgroup's threads end with) and in 64 bits for fp32 rows (they could overflow).
 // Bound: HBM.  A workgroup owns a row and holds h in registers between the two passes over it; rows too long for that are
 // read a second time (from the kept sum where there is one).  4096 x 8192 fp16 with residual, sum and 8 bits out: 46.0 us, 5.1 TB/s
 // of 7 bytes an element (a copy: 4.9); 777 x 5001 fp32 7.9 us; a single row of 4096 2.7 us, less than its launch.
@@ -126,11 +127,15 @@ rmsnorm_kernel(const RmsNormArgs g)
             }
         }
     } else {
+        double pieces = 0;                                 // (a thread adds as many as the row is long: its sum is kept in 64 bits)
         for (uint32_t k = (uint32_t)t * n; k < g.cols; k += NT * n) {
             const typename R::vec h = add(k);
             if (sum) store_chunk(sum, k, g.cols, h);
+            squares = 0;
             gather(h, load_chunk(weight, k, g.cols));
+            pieces += (double)squares;
         }
+        squares = (wide)pieces;
     }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) {
@@ -210,7 +215,7 @@ template <typename T, bool Q8> void launch_as(const RmsNormArgs& g, hipStream_t 
     // A thread per 16 bytes of an fp16 row while a workgroup has that many (4096 rows of 8192: 46.0 us, with two, four or eight
     // pieces a thread 48.5, 52.6, 58.5).  fp32 rows cost twice the arithmetic a byte: two pieces (4096 x 4096: 45.4 us, with
     // one 48.3), four where two would take 1024 threads (777 x 5001: 8.0 us against 9.7).  From 4096 pieces on (64 KB) the row
-    // is read twice: 800 x 40000 fp16 63.7 us, held eight pieces a thread 64.7.
+    // is read twice: 800 x 40000 fp16 63.9 us (63.7 with sums in fp32), held eight pieces a thread 64.7.
     using std::integral_constant;
     if (chunks <= 64) go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
     else if (chunks <= 256) go(integral_constant<int, 256>{}, integral_constant<int, 1>{});

@@ -368,7 +368,7 @@ DECX_HIP_API int decx_hip_gemm_q4_i8(const int8_t* X, const float* x_scales, con
  * sum may be x or residual, and y (in the rows' type) any of the three, at the same pitch; other overlaps are not allowed,
  * and refused where two pointers are equal.
  * Pitches in elements (of y: in elements of its own type), at least cols; any alignment of whole elements.  Sums of squares
- * are kept in fp32 (fp32 rows: 64 bits).  cols = 0 and a negative eps are refused. */
+ * are kept in fp32 (fp32 rows, and what adds up along rows above 64 KB: 64 bits).  cols = 0 and a negative eps are refused. */
 DECX_HIP_API int decx_hip_rmsnorm_f16(const uint16_t* x, const uint16_t* residual, const uint16_t* weight, uint16_t* sum,
                                       void* y, float* y_scales, uint32_t rows, uint32_t cols, uint32_t ldx, uint32_t ldr,
                                       uint32_t lds, uint32_t ldy, float eps, void* stream);

@@ -46,3 +46,23 @@ def test_codes_of_fp32_rows_next_to_a_half(hip, cols, scale):
         want = np.zeros((2, cols), np.int8)
         want[:, top], want[0, at], want[1, at] = 127, left, -left
         assert np.array_equal(dy.download(), want), (a, b, c, d)
+
+
+@pytest.mark.parametrize("cols", [40001, 1 << 20, (1 << 24) + 5])
+@pytest.mark.parametrize("value", [0.1, 0.77, 1.7])
+def test_long_rows_of_one_value(hip, cols, value):
+    """Sums whose roundings all fall to one side.  A sum of 8 squares in fp32 is off by at most 8 2^-24 of itself, the threads'
+    sums in 64 bits by next to nothing, rounding them and adding 1024 of them over lanes and wavefronts by 1 + 6 + 16; half of
+    that of the root, 6 roundings behind it: 22 2^-24."""
+    h = float(np.float16(value))
+    row = np.full((1, cols), h, np.float16)
+    d, w = hip.DeviceMatrix(1, cols, np.float16, data=row), hip.DeviceMatrix(1, cols, np.float16, data=np.ones((1, cols), np.float16))
+    codes, scale, y = hip.DeviceMatrix(1, cols, np.int8), hip.DeviceMatrix(1, 1, np.float32), hip.DeviceMatrix(1, cols, np.float16)
+    eps = float(np.float32(1e-5))
+    hip.rmsnorm(d, w, codes, y_scales=scale, eps=eps)
+    hip.rmsnorm(d, w, y, eps=eps)
+    hip.sync()
+    rho = 1 / np.sqrt(h * h + eps)
+    assert abs(float(scale.download()[0, 0]) / (h * rho / 127) - 1) <= 22 * 2.0 ** -24
+    assert (codes.download() == 127).all()
+    assert (np.abs(y.download().astype(np.float64) / (h * rho) - 1) <= 2.0 ** -11 + 22 * 2.0 ** -24).all()
