@@ -118,6 +118,24 @@ def test_more_rows_than_a_grid_has_workgroups_for(hip, kernel, i8):
         Product(hip, M, 2, 3, 128, False, i8, c=c, ldx=1).run(kernel, ldy=1)
 
 
+@pytest.mark.parametrize("kernel,M", [(ROWS_16_NARROW, 3), (ROWS_16, 9), (ROWS_16_WIDE, 13), (ROWS_32_NARROW, 18), (ROWS_32, 31), (ROWS_64_NARROW, 50), (ROWS_64, 70),
+                                      (TILES_64x128, 65), (TILES_64x256, 40), (TILES_128x384, 130)])
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_rows_behind_the_last_stay_as_they_were(hip, kernel, M, i8, splits):
+    if splits > 1 and kernel < TILES_64x128:
+        return
+    p = Product(hip, M, 37, 500, 64, True, i8)
+    y = hip.DeviceMatrix(M + 3, 37, np.float16, pad_value=-777.0)
+    y.upload_raw(np.full((M + 3, 37), -777.0, np.float16))
+    y.rows = M
+    p.into(y, hip.Q4Plan(kernel, splits, 4 // splits), p.room(splits) if splits > 1 else None)
+    hip.sync()
+    p.check(y)
+    y.rows = M + 3
+    assert (y.download_raw()[M:] == -777.0).all()
+
+
 # ---- ranges of K -----------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("kernel,bm,bn", TILED)

@@ -66,3 +66,41 @@ def test_long_rows_of_one_value(hip, cols, value):
     assert abs(float(scale.download()[0, 0]) / (h * rho / 127) - 1) <= 22 * 2.0 ** -24
     assert (codes.download() == 127).all()
     assert (np.abs(y.download().astype(np.float64) / (h * rho) - 1) <= 2.0 ** -11 + 22 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("t", [np.float16, np.float32])
+@pytest.mark.parametrize("q8", [False, True])
+def test_more_rows_than_a_launch_takes(hip, t, q8):
+    """2^21 rows a launch: every operand of the second one from its place on; rows behind the last stay as they were."""
+    rows, cols = (1 << 21) + 5, 3
+    rng = np.random.default_rng(8)
+    x, r = (rng.integers(-9, 10, (rows, cols)).astype(t) for _ in range(2))
+    x[:, 0], r[:, 0] = 20, 1                              # (no row of zeros)
+    w = np.array([[1, 0.5, -2]], t)
+    dx, dr, dw = hip.DeviceMatrix(rows, cols, t, 4, x), hip.DeviceMatrix(rows, cols, t, data=r), hip.DeviceMatrix(1, cols, t, data=w)
+    dh = hip.DeviceMatrix(rows + 2, cols, t, 5, pad_value=-777.0)
+    dy = hip.DeviceMatrix(rows + 2, cols, np.int8 if q8 else t, 4, pad_value=77)
+    ds = hip.DeviceMatrix(1, rows + 2, np.float32, data=np.full((1, rows + 2), -5, np.float32)) if q8 else None
+    dh.rows = dy.rows = rows
+    if q8:
+        ds.cols = rows
+    hip.rmsnorm(dx, dw, dy, residual=dr, sum_out=dh, y_scales=ds, eps=0.0)
+    hip.sync()
+    dh.rows = dy.rows = rows + 2
+    h = (x + r).astype(np.float64)
+    got = dh.download_raw()
+    assert np.array_equal(got[:rows, :cols], h) and (got[rows:] == -777.0).all() and (got[:, cols:] == -777.0).all()
+    p = h * w.astype(np.float64)
+    rho = 1 / np.sqrt((h * h).mean(1))
+    got = dy.download_raw()
+    assert (got[rows:] == 77).all() and (got[:, cols:] == 77).all()
+    if not q8:
+        some = p != 0
+        assert (np.abs(got[:rows, :cols][some] / (p * rho[:, None])[some] - 1) <= (2.0 ** -11 if t == np.float16 else 0) + 8 * 2.0 ** -24).all()
+        return
+    top = np.abs(p).max(1)
+    exact = 127 * p / top[:, None]                         # quotients of small whole numbers: in 64 bits a half is a half
+    assert np.array_equal(got[:rows, :cols], np.rint(exact))
+    ds.cols = rows + 2
+    s = ds.download()[0]
+    assert (s[rows:] == -5).all() and (np.abs(s[:rows] / (top * rho / 127) - 1) <= 8 * 2.0 ** -24).all()
