@@ -155,11 +155,15 @@ template <bool I8> struct XRows {
 // reads, 1 KB of a tile a load, one step ahead of the products.  X comes out of the L2, where every wavefront reads other
 // columns of it.  Read in the instruction's order, 16 rows of 64 bytes a load, it would keep the L1 busy with lines; so a
 // wavefront loads whole rows (4 of 256 bytes at a time) and turns them around in LDS of its own, which nobody waits for
-// (7 x 5003 x 7001 20.6 -> 8.1 us, 32 x 8192 x 8192 18.5 -> 12.1).  Loads under no condition took 1 x 65536 x 8192 in groups of 32
-// from 60 to 55 us, 1 x 4096 x 16384 from 8.9 to 7.5, 60 x 8192 x 4096 int8 from 10.2 to 9.2; 17 x 5003 x 7001, where the rows
-// are not aligned and half of the loads have none, costs 13.6 for 13.0.
-// Bound: the codes' way out of HBM, 1 x 65536 x 8192 in groups of 32 55 us = 5.5 TB/s; small ones the launch, 1 x 4096 x 4096
-// 5.0 us; from 32 rows on the L1, through which every workgroup draws all of X (60 x 8192 x 4096 int8 9.2 us).
+// (when it came in: 7 x 5003 x 7001 20.6 -> 8.1 us, 32 x 8192 x 8192 18.5 -> 12.1).  The same of loads under no condition: 1 x 65536
+// x 8192 in groups of 32 60 -> 55 us, 1 x 4096 x 16384 8.9 -> 7.5, 60 x 8192 x 4096 int8 10.2 -> 9.2; 17 x 5003 x 7001, where the
+// rows are not aligned and half of the loads have none, 13.0 -> 13.6.
+// Now (calls; recorded and replayed they take the same, but for the smallest): 1 x 65536 x 8192 in groups of 32 53 us = 5.7 TB/s, the
+// codes' way out of HBM; 1 x 8192 x 8192 int8 7.5, 16 x 8192 x 8192 8.7, 7 x 5003 x 7001 7.7, 60 x 8192 x 4096 int8 9.1, 32 x 8192 x 8192
+// 11.7, 17 x 5003 x 7001 12.4: the launch (a kernel with nothing to do takes 1.8) and the latency of a wavefront's few column tiles,
+// one after the other, loads one step ahead; it waits 35 to 60 % of its time, while neither the vector pipe (24-46 % busy) nor the
+// L1 (0.2-0.5 accesses a cycle and CU) nor HBM is full.  1 x 4096 x 4096 takes 4.3 us traced and 3.5 from launch to launch in a
+// recorded graph; a call from Python, 5.0, is bound by the host.
 template <bool I8, int GPB, bool ZEROS, int TM, int T, int WAVES, int CH>
 __global__ void __launch_bounds__(WAVES * 64)
 __attribute__((amdgpu_waves_per_eu(TM == 1 ? 4 : 2)))
@@ -362,9 +366,13 @@ gemm_q4_rows_kernel(const GemmQ4Args g)
 // Bound: the issue port that the vector pipe shares with the matrix pipe.  A SIMD takes a v_mfma of 16 cycles every 8 issue
 // cycles at best and a vector instruction every 4; beside 96 of the former a column tile costs a wavefront of 128 x 48 about 235
 // of the latter (9 a word to widen, 4 a tile and group to scale), 128 x 64 more registers than there are, 64 x 64 365.  So the
-// large tile of 128 x 384 holds 8 wavefronts of 128 x 48: 4096 x 8192 x 8192 fp16 498 us (1105 TFLOP/s; of it 8 % for a last
-// round of three quarters, 7 % power: 460 with zeros in X), int8 329 (1670).  64 x 64 each: 520 and 353.  Holding one of a
-// SIMD's two wavefronts back by half a step, so that one widens while the other multiplies: no gain (498 -> 549, int8 340).
+// large tile of 128 x 384 holds 8 wavefronts of 128 x 48: 4096 x 8192 x 8192 fp16 490 us (1122 TFLOP/s; 498 on a slower board, of
+// that 8 % for a last round of three quarters, 7 % power: 460 with zeros in X), int8 319 (1724).  64 x 64 each: 510 and 346.
+// Groups of 64 and 32 scale two and four times the sums: 3.7 and 5.9 vector instructions a product instead of 2.5, fp16 547 and
+// 651 us.  The small tile shares what a column and group costs among four tiles of X: 1000 x 4096 x 8192 int8 in groups of 64 with
+// zero points has 15.6 vector instructions a product (8 scale, 3.5 widen, the rest looks after scales and zero points), 82 us.
+// Holding one of a SIMD's two wavefronts back by half a step, so that one widens while the other multiplies: no gain (498 -> 549,
+// int8 329 -> 340).
 template <bool I8, int GPB, bool ZEROS, int TM, int TN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64)
 __attribute__((amdgpu_waves_per_eu(TM * TN >= 16 ? 2 : 3)))
@@ -646,7 +654,7 @@ template <bool I8, int GPB, bool ZEROS, int TM, int TN, int WM, int WN> int laun
 
 template <bool I8, int GPB, bool ZEROS> int launch_for(const GemmQ4Args& g, const GemmQ4Plan& p, hipStream_t stream)
 {
-    if (g.M <= (I8 ? 8 : 4)) {                             // (one load of X: fewer registers, less of the L1; 1 x 4096 x 16384 8.9 -> 7.5)
+    if (g.M <= (I8 ? 8 : 4)) {                             // (one load of X: fewer registers, less of the L1)
         switch (p.kernel) {
         case Q4_ROWS_16_NARROW: return launch_rows<I8, GPB, ZEROS, 1, 1, 16, 1>(g, stream);
         case Q4_ROWS_16:        return launch_rows<I8, GPB, ZEROS, 1, 2, 16, 1>(g, stream);
@@ -684,15 +692,18 @@ template <bool I8, int GPB> int launch_as(const GemmQ4Args& g, const GemmQ4Plan&
 
 // Which kernel, and how many ranges K is cut into.
 // Up to 16 rows the codes decide alone.  One row tile of W per workgroup where there are no more than 256 (a workgroup per CU:
-// 1 x 4096 x 16384 7.3 us, with two 9.8), else two, which halves what X costs (16 x 8192 x 8192 9.0 us, with one 11.4); 16
-// wavefronts per workgroup while there are few of them (7 x 5003 x 7001 7.9 us, with 8 9.4), 8 from 256 on (1 x 65536 x 8192
-// 53 us, with 16 61; 1 x 11008 x 4096 int8 6.1, with 16 7.3; 16 x 8192 x 8192 8.4, with 16 9.0).
-// Beyond, by the time that each is expected to take: the figures below, microseconds, from sweeps of 100 to 4096 rows against
-// 1024 to 11000 columns.  A kernel of few rows takes `step` per column tile of a wavefront and round of 256 workgroups; a tiled
+// 1 x 4096 x 16384 7.5 us, with two 10.2), else two, which halves what X costs (16 x 8192 x 8192 with 16 wavefronts 9.2 us, with
+// one 11.5; 7 x 5003 x 7001 7.7, with one 9.9); 16 wavefronts per workgroup while there are few of them (7 x 5003 x 7001 7.7 us, with
+// 8 8.4), 8 from 256 on (1 x 65536 x 8192 in groups of 32 53 us, with 16 61; 1 x 11008 x 4096 int8 6.1, with 16 7.6; 16 x 8192 x 8192
+// 8.7, with 16 9.2).
+// Beyond, by the time that each is expected to take: the figures in the code, microseconds, from sweeps of 100 to 4096 rows against
+// 1024 to 11000 columns.  (Zero points are left out of it: they add 3 instructions a word, and 1000 x 4096 x 8192 int8 in groups of
+// 64 is expected to take 64 us and takes 82 with them.)  A kernel of few rows takes `step` per column tile of a wavefront and round of 256 workgroups; a tiled
 // one `alone` per column tile with one workgroup on a CU, `full` with as many as it holds.  Ranges pay for storing and reading
 // their sums (7 MB/us) and a second launch; groups smaller than 128 for more sums to scale.  fp16: 128 x 8192 x 8192 on tiles of
-// 64 x 128 in 4 ranges 28.8 us, whole 55, few-rows kernel 39.6; 100 x 4096 x 4096: 14.0, 29.6, 11.9; 2048 x 4096 x 4096: 64 x 256
-// tiles 70.8 us, 64 x 128 81, 128 x 384 82; 4096 x 8192 x 8192: 521, 574, 503 (int8 356, 380, 329).
+// 64 x 128 in 4 ranges 27.0 us, whole 55.0, few-rows kernel 37.9 (int8 22.8, 45.2, 25.0); 100 x 4096 x 4096 in 8 ranges 13.9, in 4
+// 13.9, whole 29.6, few-rows kernel 19.3; 60 x 8192 x 4096 int8 on the few-rows kernel 9.2, tiles in 4 ranges 13.1; 2048 x 4096 x 4096:
+// 64 x 256 tiles 67.9 us, 64 x 128 77.0, 128 x 384 83.1; 4096 x 8192 x 8192: 510, 562, 492 (int8 346, 375, 319).
 GemmQ4Plan plan_gemm_q4(bool i8, uint32_t group, uint32_t M, uint32_t N, uint32_t K, size_t workspace_bytes)
 {
     const uint32_t nt = (N + kQ4TileRows - 1) / kQ4TileRows, kt = (K + kQ4TileCols - 1) / kQ4TileCols;

@@ -6,9 +6,11 @@
 //
 // over the group's columns; scale is computed in fp32 and held in fp16, and what follows uses the held one.  Halves round to
 // even, and a quotient next to a half is decided exactly, so that a code never depends on how a quotient was rounded.
-// Bound: HBM (N K elements in, half a byte each out), with the vector pipe close behind: about ten instructions a weight.  A wavefront makes one tile: a lane reads 8 adjacent columns of its row
-// four times (a row's 4 lanes cover 64 or 128 bytes in a row), the extremes of a group meet over those 4 lanes, and the tile
-// is stored 16 bytes per lane, 1 KB in a row.
+// A wavefront makes one tile: whole rows of it turned around in LDS, so that a lane holds 8 adjacent columns of its row four times,
+// the extremes of a group met over the row's 4 lanes, and the tile stored 16 bytes per lane, 1 KB in a row.
+// Bound: 4096 x 4096 fp16 to 4 bits 12-15 us traced, 42 MB at 2.9-3.4 TB/s: a wavefront's one chain of load, extremes, codes and store (it
+// waits 59 % of its time; the vector pipe, about ten instructions a weight, is half busy).  5003 x 7001 fp32 in groups of 32 with
+// zero points 43.5 us, 3.9 TB/s.  Back to fp32: 13.2 and 30.1 us, HBM (5.7 and 5.4 TB/s).
 #include "gemm_q4.hpp"
 
 namespace decx_hip {

@@ -8,8 +8,9 @@
 // Sums of squares are kept in fp32 for fp16 rows (a row cannot overflow it; of rows that are read twice only those of 8 elements and
 // what a workgroup's threads end with) and in 64 bits for fp32 rows (they could overflow).
 // Bound: HBM.  A workgroup owns a row and holds h in registers between the two passes over it; rows too long for that are
-// read a second time (from the kept sum where there is one).  4096 x 8192 fp16 with residual, sum and 8 bits out: 46.0 us, 5.1 TB/s
-// of 7 bytes an element (a copy: 4.9); 777 x 5001 fp32 7.9 us; a single row of 4096 2.7 us, less than its launch.
+// read a second time (from the kept sum where there is one).  4096 x 8192 fp16 with residual, sum and 8 bits out: 45.9 us, 5.1 TB/s
+// of 7 bytes an element (the calibration copy: 5.7); 777 x 5001 fp32 7.9 us; a single row of 4096 2.6 us, where a kernel with next
+// to nothing to do takes 1.8.
 #include "gemm_q4.hpp"
 
 namespace decx_hip {
