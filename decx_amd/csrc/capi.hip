@@ -121,7 +121,12 @@ void commit_split_counters(uint64_t ticket)
     if (d >= 0 && d < kMaxDevices && g_rings[d]) g_rings[d]->commit(g_ring_runtime, ticket);
 }
 
-inline int hip_rc(hipError_t e) { return (int)e; }
+// An error is reported once: what the runtime keeps of it would be taken for that of the next launch.
+inline int hip_rc(hipError_t e)
+{
+    if (e != hipSuccess) (void)hipGetLastError();
+    return (int)e;
+}
 inline hipStream_t as_stream(void* s) { return (hipStream_t)s; }
 
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }

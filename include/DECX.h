@@ -482,7 +482,8 @@ _DECX_API_ DH Conv2D(GPU_Tensor& src, GPU_TensorArray& kernel, GPU_Tensor& dst, 
                      const extend_label extend = _EXTEND_NONE_);
 
 /* ---- a linear layer with weights in 4 bits, and the norm in front of it (no counterpart in the original library).
- * All return when the result is complete; a call that fails its checks leaves its outputs as they were. */
+ * All return when the result is complete; a call that fails its checks leaves its outputs as they were.  Inputs that were given a
+ * type of another size (Reinterpret) are refused. */
 
 /* dst <- src (fp32 or fp16, outputs x inputs) in 4 bits: a scale, and with zeros a zero point, for every `group` (32, 64
  * or 128) columns of a row; decx_hip.h has the formulas (decx_hip_q4_quantize_*). */
